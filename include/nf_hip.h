@@ -43,6 +43,11 @@ extern "C" {
 #define NF_AFFINE_INTERLEAVED 0 /* params[b,2d]=unconstrained scale, [b,2d+1]=shift  (transforms.py:561-566) */
 #define NF_AFFINE_BLOCKED 1     /* params[b,d]=shift, params[b,D+d]=unconstrained scale (transforms.py:328-333) */
 
+/* element types of the entry points that take activations of several types (a separate list from the matrix modes) */
+#define NF_ELEM_F32 0
+#define NF_ELEM_BF16 1
+#define NF_ELEM_F16 2
+
 /* ABI version: major*100 + minor. */
 int nf_version(void);
 
@@ -634,6 +639,27 @@ int nf_maf_reverse_step_bwd(const double* x, int64_t x_row_stride, const double*
                             double* grad_x, int64_t grad_x_row_stride, double* grad_made_out,
                             int64_t grad_out_row_stride, double* grad_z_old, int64_t grad_z_old_row_stride, int64_t B,
                             int D, int dim, int reverse_input, void* stream);
+
+/* ---- layer normalisation (no reference counterpart: a conditioner norm that, unlike BatchNorm, couples no samples) ----
+ * Over the last axis of [rows, features], every sum in fp32:
+ *   forward   mu = mean x, r = 1 / sqrt(mean (x - mu)^2 + eps), y = (x - mu) r weight + bias
+ *   backward  u = grad_y weight, xh = (x - mu) r:  grad_x = r (u - mean u - xh mean(u xh)),
+ *             grad_weight = sum_rows grad_y xh, grad_bias = sum_rows grad_y
+ * x, y, grad_y, grad_x have the element type `elem` and their own row strides (any alignment of the element; an input's
+ * stride may be 0); weight / bias (NULL = 1 / 0), mean, rstd and the sums are fp32.  features >= 1. */
+
+/* mean / rstd [rows]: kept for the backward pass, both or neither. */
+int nf_layer_norm_fwd(const void* x, int64_t x_row_stride, const float* weight, const float* bias, void* y,
+                      int64_t y_row_stride, float* mean, float* rstd, int64_t rows, int features, double eps, int elem,
+                      void* stream);
+/* Bytes of the caller-owned workspace that grad_weight / grad_bias need (4-byte aligned). */
+size_t nf_layer_norm_bwd_workspace_bytes(int64_t rows, int features, int elem);
+/* grad_x, grad_weight, grad_bias: any of them NULL.  The sums are WRITTEN (zeros for rows = 0), in a fixed order: the
+ * same inputs give the same bits. */
+int nf_layer_norm_bwd(const void* grad_y, int64_t grad_y_row_stride, const void* x, int64_t x_row_stride,
+                      const float* mean, const float* rstd, const float* weight, void* grad_x,
+                      int64_t grad_x_row_stride, float* grad_weight, float* grad_bias, void* workspace,
+                      size_t workspace_bytes, int64_t rows, int features, int elem, void* stream);
 
 /* ---- diagnostics (no reference counterpart): what this device sustains, printed by bench.py beside the
  *      nominal roofline peaks ------------------------------------------------------------------------- */

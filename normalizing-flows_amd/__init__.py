@@ -4,6 +4,7 @@ from . import _lib
 from ._lib import invalidate_weight_caches
 from .made import MADE, MaskedLinear, DenseLinear, MaskedResidualBlock, MaskedFeedforwardBlock, \
     set_matmul_dtype, get_matmul_dtype
+from .norm import LayerNorm, layer_norm
 from .resnet import ResidualNet, ResidualBlock
 from .transforms import CompositeTransform, AutoregressiveTransform, MaskedAffineAutoregressiveTransform, \
     MaskedPiecewiseRationalQuadraticAutoregressiveTransform, MaskedPiecewiseLinearAutoregressiveTransform, \

@@ -20,6 +20,14 @@
 #define NF_AFFINE_INTERLEAVED 0  // params[b, 2d] = unconstrained scale, [2d+1] = shift (autoregressive)
 #define NF_AFFINE_BLOCKED 1      // params[b, d] = shift, params[b, D+d] = unconstrained scale (coupling)
 
+// element types of activations and matrices that come in several (not the matrix modes above)
+#define NF_ELEM_F32 0
+#define NF_ELEM_BF16 1
+#define NF_ELEM_F16 2
+
+static inline int nf_elem_size(int elem) { return elem == NF_ELEM_F32 ? 4 : (elem == NF_ELEM_BF16 || elem == NF_ELEM_F16) ? 2 : 0; }
+static inline bool nf_aligned(const void* p, int size) { return ((uintptr_t)p & (size - 1)) == 0; }
+
 static inline int nf_launch_status() {
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? NF_OK : (int)e;

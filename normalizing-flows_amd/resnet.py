@@ -2,7 +2,8 @@
 
 Same constructor, submodule names and `hidden_features` attribute as the reference; each layer is
 the fused MFMA kernel of ``made.py`` with no mask (ReLU / eval-BatchNorm prologue, bias + skip
-epilogue inside the kernel).
+epilogue inside the kernel).  `use_layer_norm` (no reference counterpart) puts ``LayerNorm`` where `use_batch_norm` puts
+BatchNorm.
 """
 import torch
 from torch import nn
@@ -10,17 +11,24 @@ from torch.nn import functional as F, init
 
 from . import _lib
 from .made import DenseLinear, _bn_scale_shift, _bn_through_torch, _check_activation, _is_relu
+from .norm import LayerNorm
 
 
 class ResidualBlock(nn.Module):
-    """x + L1(relu(BN1?(L0(relu(BN0?(x)))))) (reference resnet.py:9-57)."""
+    """x + L1(relu(N1?(L0(relu(N0?(x)))))), N BatchNorm or LayerNorm (reference resnet.py:9-57)."""
+    use_layer_norm = False          # (blocks pickled before the option existed have no attribute of their own)
 
     def __init__(self, features, context_features, activation=F.relu, dropout_probability=0.,
-                 use_batch_norm=False, zero_initialization=True):
+                 use_batch_norm=False, zero_initialization=True, use_layer_norm=False):
         super().__init__()
         _check_activation(activation)
+        if use_batch_norm and use_layer_norm:
+            raise ValueError('use_batch_norm and use_layer_norm exclude each other')
         self.activation = activation
         self.use_batch_norm = use_batch_norm
+        self.use_layer_norm = use_layer_norm
+        if use_layer_norm:
+            self.layer_norm_layers = nn.ModuleList([LayerNorm(features) for _ in range(2)])
         if use_batch_norm:
             self.batch_norm_layers = nn.ModuleList([nn.BatchNorm1d(features, eps=1e-3) for _ in range(2)])
         if context_features is not None:
@@ -31,29 +39,33 @@ class ResidualBlock(nn.Module):
             init.uniform_(self.linear_layers[-1].weight, -1e-3, 1e-3)
             init.uniform_(self.linear_layers[-1].bias, -1e-3, 1e-3)
 
+    def _norms(self):
+        if self.use_layer_norm:
+            return self.layer_norm_layers
+        return self.batch_norm_layers if self.use_batch_norm else (lambda t: t, lambda t: t)
+
     def forward(self, inputs, context=None):
         s0 = h0 = s1 = h1 = None
         if not _is_relu(self.activation):
             # general activation (resnet.py:38-57 op for op): the callable between the layers' launches
-            temps = self.batch_norm_layers[0](inputs) if self.use_batch_norm else inputs
-            temps = self.linear_layers[0].fused(self.activation(temps))
-            if self.use_batch_norm:
-                temps = self.batch_norm_layers[1](temps)
-            temps = self.dropout(self.activation(temps))
+            norms = self._norms()
+            temps = self.linear_layers[0].fused(self.activation(norms[0](inputs)))
+            temps = self.dropout(self.activation(norms[1](temps)))
             if context is None:
                 return self.linear_layers[1].fused(temps, residual=inputs)
             return inputs + self.linear_layers[1].fused(temps) * torch.sigmoid(self.context_layer(context))
         if self.training and self.dropout.p > 0:
-            # drop(act(BN1?(.))) in train() mode (resnet.py:44-50): torch's dropout between the two layers
-            bn = self.batch_norm_layers if self.use_batch_norm else (lambda t: t, lambda t: t)
-            temps = bn[1](self.linear_layers[0].fused(bn[0](inputs), relu_in=True))
+            # drop(act(N1?(.))) in train() mode (resnet.py:44-50): torch's dropout between the two layers
+            norms = self._norms()
+            temps = norms[1](self.linear_layers[0].fused(norms[0](inputs), relu_in=True))
             temps = self.dropout(torch.relu(temps))
             if context is None:
                 return self.linear_layers[1].fused(temps, residual=inputs)
             return inputs + self.linear_layers[1].fused(temps) * torch.sigmoid(self.context_layer(context))
-        if self.use_batch_norm and _bn_through_torch(self, inputs):
-            temps = self.linear_layers[0].fused(self.batch_norm_layers[0](inputs), relu_in=True)
-            temps = self.batch_norm_layers[1](temps)
+        if self.use_layer_norm or (self.use_batch_norm and _bn_through_torch(self, inputs)):
+            # (the norm's own launch; the ReLU behind it is the next layer's prologue)
+            norms = self._norms()
+            temps = norms[1](self.linear_layers[0].fused(norms[0](inputs), relu_in=True))
         else:
             if self.use_batch_norm:
                 s0, h0 = _bn_scale_shift(self.batch_norm_layers[0])
@@ -69,7 +81,7 @@ class ResidualNet(nn.Module):
     """initial linear -> residual blocks -> final linear (reference resnet.py:60-100)."""
 
     def __init__(self, in_features, out_features, hidden_features, context_features=None, num_blocks=2,
-                 activation=F.relu, dropout_probability=0., use_batch_norm=False):
+                 activation=F.relu, dropout_probability=0., use_batch_norm=False, use_layer_norm=False):
         super().__init__()
         self.hidden_features = hidden_features
         self.context_features = context_features
@@ -77,7 +89,8 @@ class ResidualNet(nn.Module):
         self.initial_layer = DenseLinear(first_in, hidden_features)
         self.blocks = nn.ModuleList([
             ResidualBlock(features=hidden_features, context_features=context_features, activation=activation,
-                          dropout_probability=dropout_probability, use_batch_norm=use_batch_norm)
+                          dropout_probability=dropout_probability, use_batch_norm=use_batch_norm,
+                          use_layer_norm=use_layer_norm)
             for _ in range(num_blocks)])
         self.final_layer = DenseLinear(hidden_features, out_features)
 
@@ -114,9 +127,10 @@ class ResidualNet(nn.Module):
         return torch.is_grad_enabled() and (inputs.requires_grad or any(p.requires_grad for p in self.parameters()))
 
     def hidden_stack_fusable(self, inputs, context=None):
-        """One launch for initial layer + blocks (nf_resnet_hidden_fwd): inference, no context, ReLU,
+        """One launch for initial layer + blocks (nf_resnet_hidden_fwd): inference, no context, ReLU, no LayerNorm,
         hidden width a multiple of 32 up to 128."""
         return (context is None and self.context_features is None and not self.records_grad(inputs)
+                and not any(b.use_layer_norm for b in self.blocks)
                 and not any(b.training and (b.use_batch_norm or b.dropout.p > 0) for b in self.blocks)
                 and all(_is_relu(b.activation) for b in self.blocks)
                 and _lib.resnet_hidden_supported(self.initial_layer.in_features, self.hidden_features))
