@@ -661,6 +661,30 @@ int nf_layer_norm_bwd(const void* grad_y, int64_t grad_y_row_stride, const void*
                       int64_t grad_x_row_stride, float* grad_weight, float* grad_bias, void* workspace,
                       size_t workspace_bytes, int64_t rows, int features, int elem, void* stream);
 
+/* ---- orthogonalised updates (no reference counterpart: what an optimizer of a conditioner's weight matrices needs) ----
+ * G (rows x cols) -> X with the singular vectors of G and singular values near 1, by `steps` Newton-Schulz products:
+ *   X = G / (|G|_F + eps);  steps times  S = X X^T, X = a X + (b S + c S S) X,  a, b, c = 3.4445, -4.7750, 2.0315
+ * on the smaller side (rows > cols: on G^T).  Products of fp32 accuracy on the fp16 matrix pipe; the norm in fp64.  A zero
+ * matrix gives zeros; a NaN or infinity anywhere in a matrix makes all of that matrix NaN, and no other. */
+
+/* Bytes of the caller-owned workspace (16-byte aligned); 0 for count = 0 or sizes outside 1 .. 2^20 (count: 65535). */
+size_t nf_orthogonalize_workspace_bytes(int64_t count, int rows, int cols);
+/* `count` matrices of type `elem`, matrix i at matrices + i * matrix_stride with contiguous rows row_stride apart (strides
+ * in elements; an input's may be 0).  out: the same type, another buffer than `matrices`. */
+int nf_orthogonalize(const void* matrices, int64_t matrix_stride, int64_t row_stride, void* out,
+                     int64_t out_matrix_stride, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                     int64_t count, int rows, int cols, int steps, double eps, int elem, void* stream);
+
+/* One Muon step of `count` contiguous fp32 matrices, in place (host arrays of device pointers and sizes):
+ *   M = momentum M + grad;  U = grad + momentum M (nesterov) or M;  O = U orthogonalised as above;
+ *   param = (1 - lr weight_decay) param - lr sqrt(max(1, rows / cols)) O
+ * params and momenta must not overlap each other or the grads.  The workspace is that of the largest batch that one
+ * sequence of launches takes (48 matrices, 8 shapes); 0 bytes mean sizes outside 1 .. 2^20. */
+size_t nf_muon_workspace_bytes(const int* rows, const int* cols, int count);
+int nf_muon_update(float* const* params, const float* const* grads, float* const* momenta, const int* rows,
+                   const int* cols, int count, double lr, double momentum, int nesterov, double weight_decay, int steps,
+                   double eps, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- diagnostics (no reference counterpart): what this device sustains, printed by bench.py beside the
  *      nominal roofline peaks ------------------------------------------------------------------------- */
 

@@ -11,6 +11,7 @@ from .transforms import CompositeTransform, AutoregressiveTransform, MaskedAffin
     MaskedPiecewiseQuadraticAutoregressiveTransform, MaskedPiecewiseCubicAutoregressiveTransform, \
     PiecewiseCubicCouplingTransform, CouplingTransform, AffineCouplingTransform, \
     PiecewiseRationalQuadraticCouplingTransform, PiecewiseRationalQuadraticCDF, PiecewiseCubicCDF
+from .optim import Muon, muon_update, orthogonalize
 from . import parallel, metrics
 from .checkpoint import save_checkpoint, load_checkpoint
 from .flows import MaskedAutoregressiveFlow, SimpleMADE, SimpleMaskedLinear, apply_flow_to_samples, \

@@ -26,6 +26,14 @@ _lib = None
 
 _c = ctypes
 _SIGNATURES = {
+    'nf_orthogonalize_workspace_bytes': (_c.c_size_t, [_c.c_int64, _c.c_int, _c.c_int]),
+    'nf_orthogonalize': (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p,
+                                    _c.c_size_t, _c.c_int64, _c.c_int, _c.c_int, _c.c_int, _c.c_double, _c.c_int,
+                                    _c.c_void_p]),
+    'nf_muon_workspace_bytes': (_c.c_size_t, [_c.c_void_p, _c.c_void_p, _c.c_int]),
+    'nf_muon_update': (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_double,
+                                  _c.c_double, _c.c_int, _c.c_double, _c.c_int, _c.c_double, _c.c_void_p, _c.c_size_t,
+                                  _c.c_void_p]),
     'nf_layer_norm_fwd': (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64,
                                      _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_double, _c.c_int, _c.c_void_p]),
     'nf_layer_norm_bwd_workspace_bytes': (_c.c_size_t, [_c.c_int64, _c.c_int, _c.c_int]),
@@ -1567,6 +1575,44 @@ def layer_norm_bwd(grad_y, x, mean, rstd, weight=None, want_x=True, want_weight=
         _check(lib.nf_layer_norm_bwd(gp, gs, xp, xs, mean.data_ptr(), rstd.data_ptr(), _ptr(weight), _ptr(gx), n, _ptr(gw),
                                      _ptr(gb), _ptr(ws), nbytes, rows, n, elem, _stream()), 'nf_layer_norm_bwd')
     return gx, gw, gb
+
+
+# ------------------------------------------------------------------------------------------------ matrix updates
+MAX_SIDE = 2 ** 20                       # rows and columns of a matrix, and ...
+MAX_MATRICES = 65535                     # ... matrices of one call, that nf_orthogonalize takes
+WORKSPACE_BYTES = 8 << 30                # what one call's workspace may take before a batch is cut (a single matrix may take more)
+
+
+def orthogonalize(g, steps, eps):
+    """g [count, rows, cols] (fp32, bf16 or fp16; contiguous rows) -> its orthogonalised matrices, same type."""
+    lib = load()
+    count, rows, cols = (int(n) for n in g.shape)
+    out = torch.empty(count, rows, cols, dtype=g.dtype, device=g.device)
+    one = lib.nf_orthogonalize_workspace_bytes(1, rows, cols)
+    per = max(1, min(count, MAX_MATRICES, WORKSPACE_BYTES // max(1, one)))
+    ws = torch.empty(lib.nf_orthogonalize_workspace_bytes(per, rows, cols), dtype=torch.uint8, device=g.device)
+    ms = g.stride(0) if count > 1 else 0
+    rs = g.stride(1) if rows > 1 else cols
+    with torch.cuda.device(g.device):
+        for at in range(0, count, per):
+            part, to = g[at:at + per], out[at:at + per]
+            _check(lib.nf_orthogonalize(part.data_ptr(), ms, rs, to.data_ptr(), rows * cols, cols, ws.data_ptr(), ws.numel(),
+                                        part.shape[0], rows, cols, steps, eps, NF_ELEM[g.dtype], _stream()),
+                   'nf_orthogonalize')
+    return out
+
+
+def muon_update(params, grads, momenta, lr, momentum, nesterov, weight_decay, steps, eps):
+    """One Muon step in place over contiguous fp32 matrices of one device."""
+    lib = load()
+    n = len(params)
+    rows, cols = ((_c.c_int * n)(*(int(p.shape[d]) for p in params)) for d in (0, 1))
+    ptrs = [(_c.c_void_p * n)(*(t.data_ptr() for t in ts)) for ts in (params, grads, momenta)]
+    device = params[0].device
+    ws = torch.empty(lib.nf_muon_workspace_bytes(rows, cols, n), dtype=torch.uint8, device=device)
+    with torch.cuda.device(device):
+        _check(lib.nf_muon_update(*ptrs, rows, cols, n, lr, momentum, int(nesterov), weight_decay, steps, eps,
+                                  ws.data_ptr(), ws.numel(), _stream()), 'nf_muon_update')
 
 
 # ------------------------------------------------------------------------------------------------

@@ -1,0 +1,405 @@
+"""nf.orthogonalize, nf.muon_update and nf.Muon against the formula in 64 bits.
+
+Tolerance: the iteration lifts an error of a step by up to 3.98 per step (the largest slope of its polynomial), so it is
+counted by running it.  `spread` runs the iteration in float64 a second time with every stored value and every product
+moved by the roundings that the kernels make there, drawn at random:
+  * X, S and b S + c S S are kept as two fp16 terms: 2^-23 of the value, and the products leave out lo lo: 2^-22;
+  * a product over K is 3 K / 16 fp32 accumulations of 16 terms each, one rounding 2^-24 of the running sum; sums of one
+    sign grow with the result, others like the root of the sum of squares:
+    2^-24 sqrt(3 K / 16 + 16) (|C| + sqrt((P P) (Q Q)^T)).
+Independent roundings of this size give a Frobenius distance like `spread`'s; four times it is the tolerance, plus half a
+step of the result's type.  One wrong element of a 1000 x 1000 result is 1e-3 of its norm, the tolerance about 1e-5."""
+import math
+
+import pytest
+import torch
+
+import normalizing_flows_amd as nf
+
+A, B, C = 3.4445, -4.7750, 2.0315
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def iterate(g, steps=5, eps=1e-7, gen=None):
+    """The formula in float64 on the device; with `gen`, moved by the rounding model of the kernels."""
+    g = g.double()
+    if g.shape[-2] > g.shape[-1]:
+        return iterate(g.mT, steps, eps, gen).mT
+
+    def noise(like):
+        return torch.randn(like.shape, dtype=torch.float64, device=like.device, generator=gen)
+
+    def kept(x):
+        return x if gen is None else x * (1 + 1.5 * 2.0 ** -22 * noise(x))
+
+    def times(p, q):
+        c = p @ q
+        if gen is None:
+            return c
+        k = p.shape[-1]
+        return c + 2.0 ** -24 * math.sqrt(3 * k / 16 + 16) * (c.abs() + ((p * p) @ (q * q)).sqrt()) * noise(c)
+
+    x = kept(g / (g.norm(dim=(-2, -1), keepdim=True) + eps))
+    for _ in range(steps):
+        s = kept(times(x, x.mT.contiguous()))
+        r = kept(B * s + C * times(s, s))
+        x = kept(A * x + times(r, x))
+    return x
+
+
+def norm(x):
+    return x.double().flatten(-2).norm(dim=-1)
+
+
+def tolerance(g, want, kind, steps=5, eps=1e-7):
+    gen = torch.Generator(device=g.device).manual_seed(77)
+    spread = norm(iterate(g, steps, eps, gen) - want)
+    n = want.shape[-2] * want.shape[-1]
+    tiny = torch.finfo(kind).tiny * torch.finfo(kind).eps * math.sqrt(n)
+    return 4 * spread + torch.finfo(kind).eps / 2 * norm(want) + tiny
+
+
+def check(got, g, kind, steps=5, eps=1e-7):
+    want = iterate(g, steps, eps)
+    assert got.shape == g.shape and got.dtype == kind
+    over = norm(got.double() - want) - tolerance(g, want, kind, steps, eps)
+    assert bool((over <= 0).all()), over.max().item()
+
+
+def gradients(shape, seed, scale=1e-3, device='cuda'):
+    """A few strong directions over a noise floor."""
+    *batch, m, n = shape
+    gen = torch.Generator().manual_seed(seed)
+    rank = max(1, min(m, n) // 8)
+    g = torch.randn(*batch, m, rank, generator=gen) @ torch.randn(*batch, rank, n, generator=gen) / math.sqrt(rank)
+    return (scale * (g + 0.1 * torch.randn(*batch, m, n, generator=gen))).to(device)
+
+
+# ---------------------------------------------------------------------------------------------- CPU: what is refused
+def test_refusals():
+    with pytest.raises(RuntimeError, match='GPU'):
+        nf.orthogonalize(torch.zeros(2, 3))
+    p = torch.nn.Parameter(torch.zeros(3))
+    with pytest.raises(ValueError):
+        nf.Muon([p])
+    with pytest.raises(ValueError):
+        nf.Muon([torch.nn.Parameter(torch.zeros(2, 3, dtype=torch.float64))])
+    m = torch.nn.Parameter(torch.zeros(2, 3))
+    for bad in (dict(lr=-1.), dict(momentum=1.), dict(momentum=-0.1), dict(weight_decay=float('nan')), dict(steps=0),
+                dict(steps=2.5), dict(eps=float('inf'))):
+        with pytest.raises(ValueError):
+            nf.Muon([m], **bad)
+    with pytest.raises(ValueError):
+        nf.muon_update([m], [m], [], 0.1)
+    with pytest.raises(RuntimeError, match='GPU'):
+        nf.muon_update([m], [m], [m], 0.1)
+    nf.muon_update([], [], [], 0.1)                     # nothing to do
+    opt = nf.Muon([m])
+    with pytest.raises(ValueError):
+        opt.add_param_group({'params': [p]})
+    assert len(opt.param_groups) == 1
+    opt.step()                                          # no gradients: nothing happens
+
+
+def test_argument_errors_before_launch():
+    lib = nf._lib.load()
+    one = 1 << 12                                       # (a non-NULL pointer that nothing reads: every call is refused)
+    need = lib.nf_orthogonalize_workspace_bytes(2, 33, 70)
+    # norms; X and twice X^T of 2 x 3 cells, S and R of 2 x 2 cells, 4 KB each
+    assert need == 2 * 256 * 8 + 2 * (3 * 6 + 2 * 4) * 4096
+    assert lib.nf_orthogonalize_workspace_bytes(0, 3, 3) == 0
+    assert lib.nf_orthogonalize_workspace_bytes(1, 0, 3) == 0 and lib.nf_orthogonalize_workspace_bytes(1, 3, 2 ** 20 + 1) == 0
+
+    def call(g=one, ms=33 * 70, rs=70, out=one, oms=33 * 70, ors=70, ws=one, nbytes=need, count=2, rows=33, cols=70, steps=5,
+             eps=1e-7, elem=0):
+        return lib.nf_orthogonalize(g, ms, rs, out, oms, ors, ws, nbytes, count, rows, cols, steps, eps, elem, None)
+
+    assert call(count=0) == 0
+    assert call(elem=3) == -5
+    assert call(rows=0) == -2 and call(steps=0) == -2 and call(eps=-1.0) == -2 and call(count=65536) == -2
+    assert call(g=None) == -1 and call(out=None) == -1 and call(ws=None) == -1
+    assert call(ors=69) == -3 and call(oms=33 * 70 - 1) == -3 and call(g=one + 2) == -3 and call(ws=one + 8) == -3
+    assert call(nbytes=need - 1) == -6
+
+
+def test_overlap_check():
+    from normalizing_flows_amd.optim import _check_disjoint
+    t = torch.zeros(40)
+    _check_disjoint([t[:10], t[10:20]], [t[20:30], t[25:40], t[20:30]])         # what is only read may overlap
+    for written, read in (([t[:10], t[9:12]], []), ([t[:10], t[:10]], []), ([t[5:10]], [t[:6]]), ([t[:6]], [t[5:10]]),
+                          ([t[30:35]], [t[:40], t[1:2]]), ([t[0:20], t[2:3]], [])):
+        with pytest.raises(ValueError):
+            _check_disjoint(written, read)
+
+
+# ---------------------------------------------------------------------------------------------- GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize('kind', TYPES, ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize('shape', [(1, 1), (1, 7), (7, 1), (2, 3), (31, 33), (32, 32), (2, 33, 129), (129, 33), (64, 64),
+                                   (3, 65, 640), (1000, 300), (2, 517, 1031), (5, 40, 50, 30), (700, 17, 5), (40, 8000),
+                                   (20, 512, 512)], ids=str)
+def test_orthogonalize(shape, kind):
+    g = gradients(shape, sum(shape)).to(kind)
+    out = nf.orthogonalize(g)
+    check(out, g, kind)
+    assert torch.equal(nf.orthogonalize(g), out)        # the same bits again
+
+
+@pytest.mark.gpu
+def test_large_matrix():
+    g = gradients((2500, 3001), 5)
+    check(nf.orthogonalize(g), g, torch.float32)
+
+
+@pytest.mark.gpu
+def test_steps_eps_and_scale():
+    g = gradients((70, 90), 1)
+    for steps in (1, 2, 7):
+        check(nf.orthogonalize(g, steps=steps), g, torch.float32, steps=steps)
+    check(nf.orthogonalize(g, eps=0.5), g, torch.float32, eps=0.5)
+    for scale in (1e-34, 1e-20, 1e18, 1e34):            # squares leave the range of fp32
+        h = g * 1e3 * scale
+        check(nf.orthogonalize(h, eps=0.0), h, torch.float32, eps=0.0)
+
+
+@pytest.mark.gpu
+def test_singular_values_come_near_one():
+    g = torch.randn(96, 200, generator=torch.Generator().manual_seed(3)).cuda()
+    s = torch.linalg.svdvals(nf.orthogonalize(g).double().cpu())
+    # (the quintic's fifth iterate of singular values in [0.05, 1] lies in [0.68, 1.2])
+    assert 0.65 < s.min().item() and s.max().item() < 1.21
+
+
+@pytest.mark.gpu
+def test_special_values_stay_in_their_matrix():
+    g = gradients((5, 40, 70), 2)
+    want = nf.orthogonalize(g)
+    h = g.clone()
+    h[1] = 0
+    h[2, 39, 69] = float('nan')
+    h[3, 0, 0] = float('inf')
+    out = nf.orthogonalize(h)
+    assert torch.equal(out[0], want[0]) and torch.equal(out[4], want[4])
+    assert not out[1].any()
+    assert out[2].isnan().all() and out[3].isnan().all()
+    assert nf.orthogonalize(torch.zeros(0, 3, 4, device='cuda')).shape == (0, 3, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kind', TYPES, ids=lambda t: str(t)[6:])
+def test_strides(kind):
+    g = gradients((3, 50, 77), 4).to(kind)
+    want = nf.orthogonalize(g)
+    wide = torch.zeros(3, 52, 90, dtype=kind, device='cuda')
+    wide[:, 1:51, 5:82] = g
+    assert torch.equal(nf.orthogonalize(wide[:, 1:51, 5:82]), want)
+    assert torch.equal(nf.orthogonalize(g.mT.contiguous().mT), want)
+    assert torch.equal(nf.orthogonalize(g[1].expand(4, 50, 77)), want[1].expand(4, 50, 77))
+    assert torch.equal(nf.orthogonalize(g.flip(0)[1]), want[1])
+    # the transposed matrix has the transposed result (both go through the same products)
+    assert torch.equal(nf.orthogonalize(g.mT), want.mT)
+
+
+@pytest.mark.gpu
+def test_a_batch_is_cut_where_its_workspace_ends(monkeypatch):
+    g = gradients((7, 40, 33), 6)
+    want = nf.orthogonalize(g)
+    monkeypatch.setattr(nf._lib, 'WORKSPACE_BYTES', 3 * nf._lib.load().nf_orthogonalize_workspace_bytes(1, 40, 33))
+    assert torch.equal(nf.orthogonalize(g), want)
+    monkeypatch.setattr(nf._lib, 'WORKSPACE_BYTES', 1)
+    assert torch.equal(nf.orthogonalize(g), want)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device():
+    g = torch.zeros(3, 4, device='cuda')
+    for bad in (dict(steps=0), dict(steps=101), dict(steps=True), dict(eps=-1.), dict(eps=float('nan'))):
+        with pytest.raises(ValueError):
+            nf.orthogonalize(g, **bad)
+    with pytest.raises(ValueError):
+        nf.orthogonalize(g[0])
+    with pytest.raises(ValueError):
+        nf.orthogonalize(torch.zeros(3, 0, device='cuda'))
+    with pytest.raises(TypeError):
+        nf.orthogonalize(g.double())
+    with pytest.raises(NotImplementedError):
+        nf.orthogonalize(g.requires_grad_())
+    with torch.no_grad():
+        assert not nf.orthogonalize(g).any()
+    p, q, m = (torch.zeros(4, 6, device='cuda') for _ in range(3))
+    for args in (([p], [q[:3]], [m]), ([p, p], [q, q], [m, m.clone()]), ([p], [q], [q]), ([p], [p], [m]),
+                 ([p.t()], [q.t()], [m.t()]), ([p[0]], [q[0]], [m[0]])):
+        with pytest.raises(ValueError):
+            nf.muon_update(*args, lr=0.1)
+    with pytest.raises(TypeError):
+        nf.muon_update([p.double()], [q.double()], [m.double()], lr=0.1)
+    assert not p.any() and not m.any()
+
+
+def muon_oracle(p, g, m, lr, momentum=0.95, nesterov=True, weight_decay=0., steps=5, eps=1e-7):
+    """(param, momentum, tolerance of the param) in float64."""
+    m = momentum * m.double() + g.double()
+    u = g.double() + momentum * m if nesterov else m
+    o = iterate(u, steps, eps)
+    rate = lr * math.sqrt(max(1, p.shape[0] / p.shape[1]))
+    # (three roundings of the parameter: the factor 1 - lr wd, the product with it and the sum)
+    tol = rate * tolerance(u, o, torch.float32, steps, eps) + 3 * 2.0 ** -24 * (norm(p) + rate * norm(o))
+    return (1 - lr * weight_decay) * p.double() - rate * o, m, tol
+
+
+def check_muon(shapes, seed, **kw):
+    gen = torch.Generator().manual_seed(seed)
+    ps = [0.1 * torch.randn(*s, generator=gen).cuda() for s in shapes]
+    gs = [gradients(s, seed + i) for i, s in enumerate(shapes)]
+    ms = [gradients(s, seed + 100 + i, 1e-2) for i, s in enumerate(shapes)]
+    want = [muon_oracle(p, g, m, **kw) for p, g, m in zip(ps, gs, ms)]
+    versions = [t._version for t in ps + ms]
+    keep = [g.clone() for g in gs]
+    nf.muon_update(ps, gs, ms, **kw)
+    assert all(t._version > v for t, v in zip(ps + ms, versions))
+    for p, g, m, k, (wp, wm, tol) in zip(ps, gs, ms, keep, want):
+        assert torch.equal(g, k)
+        assert bool((norm(p.double() - wp) <= tol).all()), p.shape
+        assert bool(((m.double() - wm).abs() <= 2.0 ** -23 * (wm.abs() + g.double().abs())).all()), p.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kw', [dict(lr=0.02), dict(lr=0.1, nesterov=False, weight_decay=0.3),
+                                dict(lr=0.0, momentum=0.0), dict(lr=0.5, steps=2, eps=1e-2)], ids=str)
+def test_muon_update(kw):
+    check_muon([(64, 32), (128, 128), (32, 64), (64, 32), (1, 1), (300, 20), (128, 128)], 9, **kw)
+
+
+@pytest.mark.gpu
+def test_muon_update_of_many_matrices_and_shapes():
+    """More matrices (48) and shapes (8) than one sequence of launches takes."""
+    check_muon([(8 + i % 11, 12) for i in range(60)], 3, lr=0.05)
+    check_muon([(5, 7)] * 50, 4, lr=0.05)
+
+
+@pytest.mark.gpu
+def test_muon_grads_of_other_layouts_and_empty_matrices():
+    p, g, m = torch.randn(30, 20).cuda(), gradients((20, 30), 1).t(), torch.zeros(30, 20).cuda()
+    want, wm, tol = muon_oracle(p, g, m, 0.1)
+    e = torch.zeros(0, 5, device='cuda')
+    nf.muon_update([e, p], [e.clone(), g], [e.clone(), m], lr=0.1)
+    assert bool((norm(p.double() - want) <= tol).all()) and bool(((m - wm).abs() <= 2.0 ** -23 * wm.abs()).all())
+
+
+@pytest.mark.gpu
+def test_streams():
+    g = gradients((4, 300, 200), 8)
+    h = gradients((2, 100, 450), 9)
+    want, other = nf.orthogonalize(g), nf.orthogonalize(h)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(3):                                  # two calls at work at once, each with a workspace of its own
+        with torch.cuda.stream(side):
+            a = nf.orthogonalize(g)
+        got.append((a, nf.orthogonalize(h)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want) and torch.equal(b, other) for a, b in got)
+
+
+@pytest.mark.gpu
+def test_captured_update():
+    """The whole step recorded into a graph and replayed, with eager work between the replays."""
+    shapes = [(70, 40), (64, 64), (40, 90)]
+    ps, ms = ([torch.zeros(s, device='cuda') for s in shapes] for _ in range(2))
+    gs = [gradients(s, 1) for s in shapes]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        nf.muon_update(ps, gs, ms, lr=0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        nf.muon_update(ps, gs, ms, lr=0.1)
+    eager = [[t.clone() for t in ts] for ts in (ps, ms)]
+    for seed in range(4):
+        for g, s in zip(gs, shapes):
+            g.copy_(gradients(s, seed + 20))
+        graph.replay()
+        torch.cuda.synchronize()
+        nf.muon_update(eager[0], gs, eager[1], lr=0.1)
+        for a, b in zip(ps + ms, eager[0] + eager[1]):
+            assert torch.equal(a, b), seed
+
+
+def small_flow(seed=0):
+    torch.manual_seed(seed)
+    mask = torch.arange(6) % 2
+    layers = [nf.PiecewiseRationalQuadraticCouplingTransform(
+        m, lambda i, o: nf.ResidualNet(i, o, 32, use_layer_norm=True), num_bins=8, tails='linear', tail_bound=3.)
+        for m in (mask, 1 - mask)]
+    layers.append(nf.MaskedPiecewiseRationalQuadraticAutoregressiveTransform(6, 24, num_bins=8, tails='linear', tail_bound=3.))
+    return nf.BaseNeuralSplineFlow(nf.CompositeTransform(layers), nf.StandardNormal([6])).cuda()
+
+
+def optimizers(flow):
+    mats = [p for p in flow.parameters() if p.dim() == 2]
+    return nf.Muon(mats, lr=0.02, weight_decay=0.01), \
+        torch.optim.Adam([p for p in flow.parameters() if p.dim() != 2], lr=1e-2)
+
+
+@pytest.mark.gpu
+def test_training_run_with_layer_norm_and_muon():
+    """A flow of layer-normalised coupling layers and a masked layer, trained by Muon and Adam: every Muon step is the
+    formula's on the gradients that the backward kernels left, the layers see the new weights at once, and a run resumed
+    from state dicts goes on with the same bits."""
+    flow = small_flow()
+    muon, adam = optimizers(flow)
+    x = torch.randn(256, 6, generator=torch.Generator().manual_seed(1)).cuda()
+    mats = muon.param_groups[0]['params']
+    saved = None
+    for step in range(4):
+        if step == 2:
+            saved = ({k: v.clone() for k, v in flow.state_dict().items()}, muon.state_dict(), adam.state_dict())
+            saved = (saved[0], torch.utils._pytree.tree_map(lambda t: t.clone() if torch.is_tensor(t) else t, saved[1:]))
+        muon.zero_grad()
+        adam.zero_grad()
+        loss = -flow.log_prob(x).mean()
+        loss.backward()
+        old = [p.detach().clone() for p in mats]
+        buf = [muon.state[p].get('momentum_buffer', torch.zeros_like(p)).clone() for p in mats]
+        muon.step()
+        adam.step()
+        for p, q, m in zip(mats, old, buf):
+            want, _, tol = muon_oracle(q, p.grad, m, lr=0.02, weight_decay=0.01)
+            assert p.grad.isfinite().all() and bool((norm(p.detach().double() - want) <= tol).all())
+        with torch.no_grad():
+            fresh = small_flow(5)
+            fresh.load_state_dict(flow.state_dict())
+            assert torch.equal(flow.log_prob(x), fresh.log_prob(x))         # no stale weight pack
+    other = small_flow(7)
+    other.load_state_dict(saved[0])
+    muon2, adam2 = optimizers(other)
+    muon2.load_state_dict(saved[1][0])
+    adam2.load_state_dict(saved[1][1])
+    for _ in range(2):
+        muon2.zero_grad()
+        adam2.zero_grad()
+        (-other.log_prob(x).mean()).backward()
+        muon2.step()
+        adam2.step()
+    # (the parameters of the two runs: equal up to the order of the weight-gradient atomics of the other kernels)
+    for p, q in zip(flow.parameters(), other.parameters()):
+        assert (p - q).abs().max().item() < 1e-3
+
+
+@pytest.mark.gpu
+def test_gradient_synchronizer_buckets_feed_the_step():
+    """Gradients that are views into flat buckets (any 4-byte alignment) are read where they are."""
+    flow = small_flow()
+    sync = nf.parallel.GradientSynchronizer(flow.parameters())
+    x = torch.randn(64, 6, generator=torch.Generator().manual_seed(2)).cuda()
+    muon, _ = optimizers(flow)
+    sync.zero_grad()
+    (-flow.log_prob(x).mean()).backward()
+    sync.finish()
+    mats = muon.param_groups[0]['params']
+    want = [muon_oracle(p.detach(), p.grad, torch.zeros_like(p), lr=0.02, weight_decay=0.01) for p in mats]
+    muon.step()
+    for p, (w, _, tol) in zip(mats, want):
+        assert bool((norm(p.detach().double() - w) <= tol).all())
