@@ -26,7 +26,7 @@ _lib = None
 
 _c = ctypes
 _SIGNATURES = {
-    'nf_orthogonalize_workspace_bytes': (_c.c_size_t, [_c.c_int64, _c.c_int, _c.c_int]),
+    'nf_orthogonalize_workspace_bytes': (_c.c_size_t, [_c.c_int64, _c.c_int, _c.c_int, _c.c_int]),
     'nf_orthogonalize': (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p,
                                     _c.c_size_t, _c.c_int64, _c.c_int, _c.c_int, _c.c_int, _c.c_double, _c.c_int,
                                     _c.c_void_p]),
@@ -1588,9 +1588,9 @@ def orthogonalize(g, steps, eps):
     lib = load()
     count, rows, cols = (int(n) for n in g.shape)
     out = torch.empty(count, rows, cols, dtype=g.dtype, device=g.device)
-    one = lib.nf_orthogonalize_workspace_bytes(1, rows, cols)
+    one = lib.nf_orthogonalize_workspace_bytes(1, rows, cols, NF_ELEM[g.dtype])
     per = max(1, min(count, MAX_MATRICES, WORKSPACE_BYTES // max(1, one)))
-    ws = torch.empty(lib.nf_orthogonalize_workspace_bytes(per, rows, cols), dtype=torch.uint8, device=g.device)
+    ws = torch.empty(lib.nf_orthogonalize_workspace_bytes(per, rows, cols, NF_ELEM[g.dtype]), dtype=torch.uint8, device=g.device)
     ms = g.stride(0) if count > 1 else 0
     rs = g.stride(1) if rows > 1 else cols
     with torch.cuda.device(g.device):

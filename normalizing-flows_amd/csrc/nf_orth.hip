@@ -27,6 +27,8 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float CA = 3.4445f, CB = -4.7750f, CC = 2.0315f;
 constexpr int CELL = 4096;               // bytes of a 32 x 32 cell
@@ -41,11 +43,14 @@ struct Group {
     int sm, sn;                          // cells along each
     int trans;                           // rows > columns: X = G^T
     int count, first;                    // matrices, index of the first
-    int64_t x, xt[2], s, r;              // byte offsets in the workspace; matrix i of X is at x + i * sm * sn * CELL, ...
+    int64_t x, xt[2], s;                 // byte offsets in the workspace: X, X^T (two), the slots of m x m matrices, each
+                                         // of them `count` matrices one behind the other
 };
 struct Plan {
     Group g[MAX_GROUPS];
-    int first_tile[MAX_GROUPS + 1];      // tiles of the launch, group by group
+    int first_tile[MAX_GROUPS + 1];      // workgroups of the launch, group by group
+    int parts[MAX_GROUPS];               // of the k cells of a symmetric product's tile
+    int64_t partial[MAX_GROUPS];         // offset of their accumulators, in floats
     int groups;
 };
 struct Pointers {
@@ -62,15 +67,10 @@ struct Ends {
     int nesterov;
 };
 
-__device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
-    hi = (_Float16)v;
-    lo = (_Float16)(v - (float)hi);
-}
-
 // (LDS traffic of a wave with itself: in order, but only this tells the compiler that lanes talk to each other)
 __device__ __forceinline__ void wave_sync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// Workgroups go round robin to the eight XCDs, each with an L2 of its own: XCD k gets the k-th eighth of the tiles.
+// Workgroups go round robin to the eight XCDs, each with an L2 of its own: XCD k gets the k-th eighth of a group's tiles.
 __device__ __forceinline__ int xcd_order(int id, int total) {
     const int q = total >> 3, rest = total & 7, xcd = id & 7;
     return xcd * q + (xcd < rest ? xcd : rest) + (id >> 3);
@@ -114,44 +114,33 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(Plan plan, Pointers ptr,
 }
 
 // ---- cells ---------------------------------------------------------------------------------------------------------------
-// one term pair of a cell's k block q, from / to memory: this lane's 8 values of row lane % 32, columns 16 q + 8 (lane / 32)
-__device__ __forceinline__ void store_terms(char* cell, int q, int lane, const float* v) {
-    f16x8 hi, lo;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        _Float16 h, l;
-        split(v[e], h, l);
-        hi[e] = h;
-        lo[e] = l;
-    }
-    *reinterpret_cast<f16x8*>(cell + q * 2 * PIECE + lane * 16) = hi;
-    *reinterpret_cast<f16x8*>(cell + q * 2 * PIECE + PIECE + lane * 16) = lo;
+// a value as its two terms: hi in the low half, lo in the high half of a word
+__device__ __forceinline__ uint32_t split(float v) {
+    const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
+    return (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
 }
 
-__device__ __forceinline__ void load_terms(const char* cell, int q, int lane, float* v) {
-    const f16x8 hi = *reinterpret_cast<const f16x8*>(cell + q * 2 * PIECE + lane * 16);
-    const f16x8 lo = *reinterpret_cast<const f16x8*>(cell + q * 2 * PIECE + PIECE + lane * 16);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)hi[e] + (float)lo[e];
-}
-
-// a wave's 32 x 32 floats in LDS
+// A wave's 32 x 32 words in LDS: values change between the layout of the accumulators (or of the caller's matrix) and the
+// two orientations of a cell.
 struct Sub {
-    float (*at)[33];
-    __device__ __forceinline__ void rows(int q, int lane, float* v) const {
-        const int r = lane & 31, c = 16 * q + 8 * (lane >> 5);
+    uint32_t (*at)[33];
+    // this lane's part of the cell (row lane % 32, columns 16 q + 8 (lane / 32) ..), or of its transpose, to memory
+    template <bool TRANSPOSED>
+    __device__ __forceinline__ void store(char* cell, int lane) const {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = at[r][c + e];
-    }
-    __device__ __forceinline__ void put_rows(int q, int lane, const float* v) const {
-        const int r = lane & 31, c = 16 * q + 8 * (lane >> 5);
+        for (int q = 0; q < 2; ++q) {
+            const int r = lane & 31, c = 16 * q + 8 * (lane >> 5);
+            u32x4 hi, lo;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) at[r][c + e] = v[e];
-    }
-    __device__ __forceinline__ void columns(int q, int lane, float* v) const {
-        const int r = lane & 31, c = 16 * q + 8 * (lane >> 5);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = at[c + e][r];
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t v = TRANSPOSED ? at[c + 2 * e][r] : at[r][c + 2 * e];
+                const uint32_t w = TRANSPOSED ? at[c + 2 * e + 1][r] : at[r][c + 2 * e + 1];
+                hi[e] = (v & 0xffff) | w << 16;
+                lo[e] = v >> 16 | (w & 0xffff0000);
+            }
+            *reinterpret_cast<u32x4*>(cell + q * 2 * PIECE + lane * 16) = hi;
+            *reinterpret_cast<u32x4*>(cell + q * 2 * PIECE + PIECE + lane * 16) = lo;
+        }
     }
 };
 
@@ -159,7 +148,7 @@ struct Sub {
 template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void orth_start_kernel(Plan plan, Pointers ptr, Ends io, const double* __restrict__ partial,
                                                          int blocks, double eps, char* __restrict__ ws) {
-    __shared__ float lds[4][32][33];
+    __shared__ uint32_t lds[4][32][33];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     int k = 0;
     while (k + 1 < plan.groups && (int)blockIdx.x >= plan.first_tile[k + 1]) ++k;
@@ -194,20 +183,14 @@ __global__ __launch_bounds__(256) void orth_start_kernel(Plan plan, Pointers ptr
             }
             v = (float)((double)v * scale);
         }
-        if (g.trans) sub.at[c][r] = v;
-        else sub.at[r][c] = v;
+        if (g.trans) sub.at[c][r] = split(v);
+        else sub.at[r][c] = split(v);
     }
     wave_sync();
     char* x = ws + g.x + ((int64_t)idx * cells + (int64_t)ci * g.sn + cj) * CELL;
     char* xt = ws + g.xt[0] + ((int64_t)idx * cells + (int64_t)cj * g.sm + ci) * CELL;
-    float v[8];
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        sub.rows(q, lane, v);
-        store_terms(x, q, lane, v);
-        sub.columns(q, lane, v);
-        store_terms(xt, q, lane, v);
-    }
+    sub.store<false>(x, lane);
+    sub.store<true>(xt, lane);
 }
 
 // ---- products --------------------------------------------------------------------------------------------------------------
@@ -219,201 +202,385 @@ __device__ __forceinline__ void piece_to_lds(const char* src, unsigned dst) {
                  : "=&s"(keep) : "v"(src), "s"(dst) : "memory");
 }
 
-enum { MAKE_S, MAKE_R, MAKE_X, MAKE_LAST };              // S = X X^T; R = b S + c S S; X = a X + R X; the same, result out
-enum { OUT_F32, OUT_BF16, OUT_F16, OUT_MUON };
+// A symmetric result in slot `out`: k0 (P Q^T + k1 E1 + k2 E2), the factors with the powers of two of the operands' scales
+// (P = Q = X where p is FROM_X, else slots; E1, E2: slots or NONE).  The E's are where the accumulators start from.
+constexpr int FROM_X = -1, NONE = -1;
+struct SymOp { int p, q, out, e1, e2; float k0, k1, k2; };
+struct SymOps { SymOp op[2]; };
+// X <- alpha X + T X from slot r: the accumulators start from scale_x * X (alpha with T's power of two), and out_scale takes
+// them back to X's scale
+struct MixOp { int r, to; float scale_x, out_scale; };
 
-// TI x TJ cells a workgroup, WI x WJ waves, a ring of RING k blocks in LDS
-template <int TI, int TJ, int WI, int WJ, int RING, int WHAT, int OUT>
-__global__ __launch_bounds__(WI * WJ * 64) void orth_product_kernel(Plan plan, Pointers ptr, Ends io, int to, char* __restrict__ ws) {
-    constexpr int W = WI * WJ, FI = TI / WI, FJ = TJ / WJ;
-    constexpr int STAGE = (TI + TJ) * 2 * PIECE, LOADS = (TI + TJ) * 2 / W;
-    static_assert((TI + TJ) * 2 % W == 0 && TI % WI == 0 && TJ % WJ == 0, "whole pieces and cells per wave");
-    static_assert(W * 32 * 33 * 4 <= RING * STAGE, "the epilogue reuses the ring");
-    extern __shared__ __align__(16) char lds[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = xcd_order(blockIdx.x, gridDim.x);
-    int k = 0;
-    while (k + 1 < plan.groups && tile >= plan.first_tile[k + 1]) ++k;
-    const Group& g = plan.g[k];
-    // the tile's cells
-    constexpr bool SYM = WHAT == MAKE_S || WHAT == MAKE_R;
-    const int ni = (g.sm + TI - 1) / TI, nj = SYM ? ni : (g.sn + TJ - 1) / TJ;
-    const int per = SYM ? ni * (ni + 1) / 2 : ni * nj;
-    const int in_group = tile - plan.first_tile[k], idx = in_group / per;
-    int t = in_group - idx * per, ti, tj;
-    if (SYM) {                                           // the triangle tj >= ti, row by row
-        ti = 0;
-        while (t >= ni - ti) t -= ni - ti++;
-        tj = ti + t;
-    } else {
-        ti = t / nj;
-        tj = t - ti * nj;
-    }
-    const int64_t xm = (int64_t)idx * g.sm * g.sn * CELL, sm2 = (int64_t)idx * g.sm * g.sm * CELL;
-    const int cur = to ^ 1;
-    const char* p = ws + (WHAT == MAKE_S ? g.x + xm : WHAT == MAKE_R ? g.s + sm2 : g.r + sm2);
-    const char* q = ws + (WHAT == MAKE_S ? g.x + xm : WHAT == MAKE_R ? g.s + sm2 : g.xt[cur] + xm);
-    const int kcells = WHAT == MAKE_S ? g.sn : g.sm, steps = 2 * kcells;
-    const int prows = g.sm, qrows = SYM ? g.sm : g.sn;
+// vmcnt(N) lgkmcnt(0): at most N loads on their way, all LDS reads back
+template <int N> __device__ __forceinline__ void wait_loads() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (0 << 8) | ((N >> 4) << 14));
+}
 
-    // this wave's pieces of a k block: cells past the matrix read its last ones (their results are not kept)
+// The k loop: TI x TJ cells, four waves in 2 x 2, each FI x FJ cells of 32 x 32.  A ring of RING k blocks of 16 in LDS.  Step s
+// multiplies block s from registers and meanwhile reads block s + 1 from LDS into a second set of fragments and requests
+// block s + RING into the place of block s: reads and requests go between the matrix instructions, which a single wave per
+// SIMD must issue without a pause.  `p`, `q`: the operands' cells of row 0; rows past the matrix read its last ones (their
+// results are not kept).
+template <int TI, int TJ, int RING>
+struct Ring {
+    static constexpr int FI = TI / 2, FJ = TJ / 2, STAGE = (TI + TJ) * 2 * PIECE, LOADS = (TI + TJ) / 2;
+    static constexpr int READS = 2 * (FI + FJ);
+    f32x16 acc[FI][FJ];
+    f16x8 frag_a[2][FI][2], frag_b[2][FJ][2];            // [set][cell][term]
     const char* src[LOADS];
     unsigned dst[LOADS];
-    const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-#pragma unroll
-    for (int l = 0; l < LOADS; ++l) {
-        const int piece = wave * LOADS + l, cell = piece >> 1, term = piece & 1;
-        int row = cell < TI ? ti * TI + cell : tj * TJ + cell - TI;
-        const int most = (cell < TI ? prows : qrows) - 1;
-        row = row < most ? row : most;
-        src[l] = (cell < TI ? p : q) + (int64_t)row * kcells * CELL + term * PIECE + lane * 16;
-        dst[l] = base + piece * PIECE;
+    unsigned place;                                      // of the next request
+    const char *from_a, *from_b;                         // this lane's fragments in place 0
+    unsigned next;                                       // place of the next block to read
+
+    __device__ __forceinline__ void request(int l) {
+        piece_to_lds(src[l], dst[l] + place);
+        src[l] += 2 * PIECE;
     }
-    int filled = 0;                                      // k blocks requested so far
-    auto fill = [&]() {
-        const unsigned at = (unsigned)(filled % RING) * STAGE;
+    __device__ __forceinline__ void turn(unsigned& at) { at = at == (RING - 1) * STAGE ? 0 : at + STAGE; }
+    __device__ __forceinline__ void fill() {
 #pragma unroll
-        for (int l = 0; l < LOADS; ++l) {
-            piece_to_lds(src[l], dst[l] + at);
-            src[l] += 2 * PIECE;
+        for (int l = 0; l < LOADS; ++l) request(l);
+        turn(place);
+    }
+    __device__ __forceinline__ void read(int set, int r) {                       // fragment r of READS
+        if (r < 2 * FI) frag_a[set][r >> 1][r & 1] = *reinterpret_cast<const f16x8*>(from_a + next + r * PIECE);
+        else frag_b[set][(r >> 1) - FI][r & 1] = *reinterpret_cast<const f16x8*>(from_b + next + (r - 2 * FI) * PIECE);
+    }
+    // one step: FILL requests a block, READ reads the next one
+    template <int SET, bool FILL, bool READ>
+    __device__ __forceinline__ void step() {
+        constexpr int M = 3 * FI * FJ, EACH = (READS * 3 + 2 * M - 1) / (2 * M), PER = M / LOADS;
+        int r = 0, l = 0;
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            const int term = m / (FI * FJ), i = m / FJ % FI, j = m % FJ;
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag_a[SET][i][term == 1], frag_b[SET][j][term == 0], acc[i][j], 0, 0, 0);
+            if (READ && r < READS) {                     // within the first two thirds of the products
+#pragma unroll
+                for (int e = 0; e < EACH; ++e)
+                    if (r < READS) read(SET ^ 1, r++);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (FILL && (m + 1) % PER == 0 && l < LOADS) {
+                request(l++);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        ++filled;
-    };
-    f32x16 acc[FI][FJ];
+        if (FILL) {
 #pragma unroll
-    for (int i = 0; i < FI; ++i)
-#pragma unroll
-        for (int j = 0; j < FJ; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    const int wi = wave / WJ, wj = wave - wi * WJ;
-    while (filled < RING - 1 && filled < steps) fill();
-    for (int s = 0; s < steps; ++s) {
-        // block s has landed when at most the blocks behind it are still on their way (loads return in order); then every
-        // wave is past its reads of block s - 1, whose place block s + RING - 1 takes
-        if (filled - s == RING - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * LOADS) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (filled < steps) fill();
-        const char* stage = lds + (s % RING) * STAGE + lane * 16;
-        f16x8 a[FI][2], b[FJ][2];
+            for (int e = M / PER; e < LOADS; ++e) request(e);
+            turn(place);
+        }
+        if (READ) turn(next);
+    }
+    // block s + 1 has landed when at most N requests behind it are on their way (loads return in order), and this wave's
+    // reads of block s are back; the barrier makes that true of all four waves
+    template <int N> __device__ __forceinline__ void meet() {
+        asm volatile("" ::: "memory");
+        wait_loads<N>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < FI; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) a[i][h] = *reinterpret_cast<const f16x8*>(stage + ((wi * FI + i) * 2 + h) * PIECE);
+            for (int j = 0; j < FJ; ++j)
 #pragma unroll
-        for (int j = 0; j < FJ; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) b[j][h] = *reinterpret_cast<const f16x8*>(stage + ((TI + wj * FJ + j) * 2 + h) * PIECE);
-#pragma unroll
-        for (int term = 0; term < 3; ++term)
-#pragma unroll
-            for (int i = 0; i < FI; ++i)
-#pragma unroll
-                for (int j = 0; j < FJ; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][term == 1], b[j][term == 0], acc[i][j], 0, 0, 0);
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // the ring becomes the epilogue's
+    // acc += scale * E, from the cells of E^T (rows as Q's, columns as P's): an accumulator's four rows are 8 bytes there
+    __device__ __forceinline__ void add(const char* et, int64_t row_bytes, int ci0, int cj0, int prows, int qrows, float scale) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) {
+                const int ci = ci0 + i < prows ? ci0 + i : prows - 1, cj = cj0 + j < qrows ? cj0 + j : qrows - 1;
+                const char* cell = et + cj * row_bytes + (int64_t)ci * CELL + (lane & 31) * 16 + (lane >> 5) * 8;
+                f16x4 hi[4], lo[4];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {            // rows 8 g + 4 (lane / 32) .. + 3
+                    const char* at = cell + (g >> 1) * 2 * PIECE + (g & 1) * 512;
+                    hi[g] = *reinterpret_cast<const f16x4*>(at);
+                    lo[g] = *reinterpret_cast<const f16x4*>(at + PIECE);
+                }
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[i][j][4 * g + e] = __builtin_fmaf(scale, (float)hi[g][e] + (float)lo[g][e], acc[i][j][4 * g + e]);
+                if (FI * FJ > 4) __builtin_amdgcn_sched_barrier(0);      // (all cells' loads at once would not fit the registers)
+            }
+    }
+    // k cells first .. last - 1 (at least one); `start` sets the accumulators while the first blocks are on their way
+    template <typename Start>
+    __device__ __forceinline__ void run(char* lds, const char* p, const char* q, int64_t row_bytes, int ti, int tj, int prows,
+                                        int qrows, int first, int last, Start start) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wi = wave >> 1, wj = wave & 1;
+        const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l) {
+            const int piece = wave * LOADS + l, cell = piece >> 1, term = piece & 1;
+            int row = cell < TI ? ti * TI + cell : tj * TJ + cell - TI;
+            const int most = (cell < TI ? prows : qrows) - 1;
+            row = row < most ? row : most;
+            src[l] = (cell < TI ? p : q) + row * row_bytes + (int64_t)first * CELL + term * PIECE + lane * 16;
+            dst[l] = base + piece * PIECE;
+        }
+        from_a = lds + wi * FI * 2 * PIECE + lane * 16;
+        from_b = lds + (TI + wj * FJ) * 2 * PIECE + lane * 16;
+        place = next = 0;
+        const int steps = 2 * (last - first);            // even, at least 2
+#pragma unroll
+        for (int s = 0; s < RING; ++s)
+            if (s < steps) fill();
+        start();
+        if (steps > RING) meet<(RING - 1) * LOADS>();
+        else meet<0>();
+#pragma unroll
+        for (int r = 0; r < READS; ++r) read(0, r);
+        turn(next);
+        int s = 0;
+        for (; s + RING + 1 < steps; s += 2) {
+            meet<(RING - 2) * LOADS>();
+            step<0, true, true>();
+            meet<(RING - 2) * LOADS>();
+            step<1, true, true>();
+        }
+        if (RING % 2 && s + RING < steps) {              // (an odd ring's last request)
+            meet<(RING - 2) * LOADS>();
+            step<0, true, true>();
+            meet<0>();
+            step<1, false, true>();
+            s += 2;
+        }
+        for (; s + 2 < steps; s += 2) {                  // the last blocks are all requested
+            meet<0>();
+            step<0, false, true>();
+            meet<0>();
+            step<1, false, true>();
+        }
+        meet<0>();
+        step<0, false, true>();
+        step<1, false, false>();
+        meet<0>();                                       // the ring becomes the epilogue's
+    }
+};
 
-    const Sub sub = {reinterpret_cast<float(*)[33]>(lds + wave * 32 * 33 * 4)};
-    float rate = 0.f;
-    if (WHAT == MAKE_LAST && OUT == OUT_MUON) {
-        const float rows = (float)(g.trans ? g.n : g.m), cols = (float)(g.trans ? g.m : g.n);
-        rate = io.lr * sqrtf(fmaxf(1.f, rows / cols));
+// a cell's accumulators times `scale` into sub, as term pairs or as floats
+template <bool TERMS>
+__device__ __forceinline__ void put_acc(const Sub& sub, int lane, const f32x16& acc, float scale) {
+    __builtin_amdgcn_sched_barrier(0);                   // (several cells' epilogues at once would not fit the registers)
+    wave_sync();                                         // (what was there before has been read)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const float v = acc[r] * scale;
+        sub.at[8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)][lane & 31] = TERMS ? split(v) : __builtin_bit_cast(uint32_t, v);
     }
+    wave_sync();
+}
+
+// one cell of a symmetric result at (ci, cj) and, where `mirror`, (cj, ci)
+__device__ __forceinline__ void finish_sym(const Sub& sub, const f32x16& acc, float scale, char* out, int sm, int ci, int cj,
+                                           bool mirror, int lane) {
+    put_acc<true>(sub, lane, acc, scale);
+    sub.store<false>(out + ((int64_t)ci * sm + cj) * CELL, lane);
+    if (mirror) sub.store<true>(out + ((int64_t)cj * sm + ci) * CELL, lane);
+}
+
+// the triangle tj >= ti of n x n tiles, row by row
+__device__ __forceinline__ void triangle(int t, int n, int& ti, int& tj) {
+    ti = 0;
+    while (t >= n - ti) t -= n - ti++;
+    tj = ti + t;
+}
+
+// Symmetric products: blockIdx.y picks the operation.  Where a group's k cells are cut into parts, a workgroup takes one
+// and leaves its raw accumulators in `partial`, which orth_sym_finish_kernel adds in order.
+template <int T, int RING>
+__global__ __launch_bounds__(256) void orth_sym_kernel(Plan plan, SymOps ops, float* __restrict__ partial, char* __restrict__ ws) {
+    extern __shared__ __align__(16) char lds[];
+    const SymOp& op = ops.op[blockIdx.y];
+    int k = 0;
+    while (k + 1 < plan.groups && (int)blockIdx.x >= plan.first_tile[k + 1]) ++k;
+    const Group& g = plan.g[k];
+    const int n = (g.sm + T - 1) / T, per = n * (n + 1) / 2, parts = plan.parts[k];
+    const int order = xcd_order(blockIdx.x - plan.first_tile[k], plan.first_tile[k + 1] - plan.first_tile[k]);
+    const int in_group = order / parts, part = order - in_group * parts, idx = in_group / per;
+    int ti, tj;
+    triangle(in_group - idx * per, n, ti, tj);
+    const int64_t slot = (int64_t)g.count * g.sm * g.sm * CELL;
+    char* slots = ws + g.s + (int64_t)idx * g.sm * g.sm * CELL;
+    const bool from_x = op.p == FROM_X;
+    const char* p = from_x ? ws + g.x + (int64_t)idx * g.sm * g.sn * CELL : slots + op.p * slot;
+    const char* q = from_x ? p : slots + op.q * slot;
+    const int kcells = from_x ? g.sn : g.sm;
+    const int first = (int)((int64_t)kcells * part / parts), last = (int)((int64_t)kcells * (part + 1) / parts);
+    Ring<T, T, RING> ring;
+    constexpr int F = T / 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave >> 1, wj = wave & 1;
+    const int64_t row_bytes = (int64_t)kcells * CELL;
+    ring.run(lds, p, q, row_bytes, ti, tj, g.sm, g.sm, first, last, [&]() {
+        ring.clear();
+        if (op.e1 != NONE && part == 0) ring.add(slots + op.e1 * slot, row_bytes, ti * T + wi * F, tj * T + wj * F, g.sm, g.sm, op.k1);
+        if (op.e2 != NONE && part == 0) ring.add(slots + op.e2 * slot, row_bytes, ti * T + wi * F, tj * T + wj * F, g.sm, g.sm, op.k2);
+    });
+    const Sub sub = {reinterpret_cast<uint32_t(*)[33]>(lds + wave * 32 * 33 * 4)};
 #pragma unroll
-    for (int i = 0; i < FI; ++i)
+    for (int i = 0; i < F; ++i)
 #pragma unroll
-        for (int j = 0; j < FJ; ++j) {
-            const int ci = ti * TI + wi * FI + i, cj = tj * TJ + wj * FJ + j;
-            if (ci >= prows || cj >= qrows) continue;
-            wave_sync();                                 // (the cell before this one has been read)
+        for (int j = 0; j < F; ++j) {
+            const int li = wi * F + i, lj = wj * F + j, ci = ti * T + li, cj = tj * T + lj;
+            if (ci >= g.sm || cj >= g.sm) continue;
+            if (parts > 1) {
+                float* to = partial + plan.partial[k] +
+                            (((int64_t)blockIdx.y * per * g.count * parts + order) * (T * T) + li * T + lj) * 1024 + lane * 4;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sub.at[8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)][lane & 31] = acc[i][j][r];
-            wave_sync();
-            float v[8], w[8];
-            if constexpr (SYM) {
-                char* out = ws + (WHAT == MAKE_S ? g.s : g.r) + sm2;
-                const char* s = ws + g.s + sm2;
-#pragma unroll
-                for (int side = 0; side < 2; ++side) {
-                    if (side && ti == tj) break;         // (a tile on the diagonal holds both halves)
-                    const int64_t at = ((int64_t)(side ? cj : ci) * g.sm + (side ? ci : cj)) * CELL;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (side) sub.columns(h, lane, v);
-                        else sub.rows(h, lane, v);
-                        if (WHAT == MAKE_S) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) v[e] *= 0x1p-15f;
-                        } else {
-                            load_terms(s + at, h, lane, w);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) v[e] = (CB * 0x1p-1f) * w[e] + (CC * 0x1p-16f) * v[e];
-                        }
-                        store_terms(out + at, h, lane, v);
-                    }
-                }
+                for (int r = 0; r < 4; ++r)
+                    *reinterpret_cast<float4*>(to + r * 256) = make_float4(ring.acc[i][j][4 * r], ring.acc[i][j][4 * r + 1],
+                                                                           ring.acc[i][j][4 * r + 2], ring.acc[i][j][4 * r + 3]);
             } else {
-                char* x = ws + g.x + xm + ((int64_t)ci * g.sn + cj) * CELL;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    sub.rows(h, lane, v);
-                    load_terms(x, h, lane, w);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = CA * w[e] + 0x1p-14f * v[e];
-                    sub.put_rows(h, lane, v);
-                    if (WHAT == MAKE_X) store_terms(x, h, lane, v);
-                }
-                wave_sync();
-                if constexpr (WHAT == MAKE_X) {
-                    char* xt = ws + g.xt[to] + xm + ((int64_t)cj * g.sm + ci) * CELL;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        sub.columns(h, lane, v);
-                        store_terms(xt, h, lane, v);
-                    }
-                } else {
-                    const int mat = g.first + idx;
-                    const int r0 = (g.trans ? cj : ci) * 32, c0 = (g.trans ? ci : cj) * 32;
-                    const int rows = g.trans ? g.n : g.m, cols = g.trans ? g.m : g.n;
-#pragma unroll
-                    for (int it = 0; it < 16; ++it) {
-                        const int r = it * 2 + (lane >> 5), c = lane & 31;
-                        if (r0 + r >= rows || c0 + c >= cols) continue;
-                        const float o = (g.trans ? sub.at[c][r] : sub.at[r][c]) * 0x1p-15f;
-                        if constexpr (OUT == OUT_MUON) {
-                            float* w0 = ptr.param[mat] + (int64_t)(r0 + r) * cols + c0 + c;
-                            *w0 = __builtin_fmaf(-rate, o, *w0 * io.keep);
-                        } else {
-                            const int64_t at = mat * io.out_matrix + (int64_t)(r0 + r) * io.out_row + c0 + c;
-                            if (OUT == OUT_F32) ((float*)io.out)[at] = o;
-                            else if (OUT == OUT_BF16) ((__bf16*)io.out)[at] = (__bf16)o;
-                            else ((_Float16*)io.out)[at] = (_Float16)o;
-                        }
-                    }
-                }
+                finish_sym(sub, ring.acc[i][j], op.k0, slots + op.out * slot, g.sm, ci, cj, ti != tj, lane);
             }
         }
 }
 
+// a wave a cell: the partial accumulators of a tile's parts added in order, then the cell's epilogue (plan: the groups with
+// parts only)
+template <int T>
+__global__ __launch_bounds__(256) void orth_sym_finish_kernel(Plan plan, SymOps ops, const float* __restrict__ partial,
+                                                              char* __restrict__ ws) {
+    __shared__ uint32_t lds[4][32][33];
+    const SymOp& op = ops.op[blockIdx.y];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int k = 0;
+    while (k + 1 < plan.groups && (int)blockIdx.x >= plan.first_tile[k + 1]) ++k;
+    const Group& g = plan.g[k];
+    const int n = (g.sm + T - 1) / T, per = n * (n + 1) / 2, parts = plan.parts[k];
+    const int id = (blockIdx.x - plan.first_tile[k]) * 4 + wave, in_group = id / (T * T), local = id - in_group * (T * T);
+    const int li = local / T, lj = local - li * T, idx = in_group / per;
+    int ti, tj;
+    triangle(in_group - idx * per, n, ti, tj);
+    const int ci = ti * T + li, cj = tj * T + lj;
+    if (ci >= g.sm || cj >= g.sm) return;                // (no barriers below: the waves are independent)
+    const float* from = partial + plan.partial[k] +
+                        (((int64_t)blockIdx.y * per * g.count + in_group) * parts * (T * T) + local) * 1024 + lane * 4;
+    f32x16 acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+#pragma unroll 4
+    for (int part = 0; part < parts; ++part, from += T * T * 1024) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float4 v = *reinterpret_cast<const float4*>(from + r * 256);
+            acc[4 * r] += v.x;
+            acc[4 * r + 1] += v.y;
+            acc[4 * r + 2] += v.z;
+            acc[4 * r + 3] += v.w;
+        }
+    }
+    const Sub sub = {lds[wave]};
+    const int64_t one = (int64_t)g.sm * g.sm * CELL;
+    finish_sym(sub, acc, op.k0, ws + g.s + op.out * g.count * one + idx * one, g.sm, ci, cj, ti != tj, lane);
+}
+
+enum { OUT_X, OUT_F32, OUT_BF16, OUT_F16, OUT_MUON };
+
+// X <- alpha X + T X: both orientations written (OUT_X), or the result in the caller's matrices
+template <int TI, int TJ, int RING, int OUT>
+__global__ __launch_bounds__(256, 2) void orth_mix_kernel(Plan plan, Pointers ptr, Ends io, MixOp op, char* __restrict__ ws) {
+    extern __shared__ __align__(16) char lds[];
+    int k = 0;
+    while (k + 1 < plan.groups && (int)blockIdx.x >= plan.first_tile[k + 1]) ++k;
+    const Group& g = plan.g[k];
+    const int ni = (g.sm + TI - 1) / TI, nj = (g.sn + TJ - 1) / TJ;
+    const int in_group = xcd_order(blockIdx.x - plan.first_tile[k], plan.first_tile[k + 1] - plan.first_tile[k]);
+    const int idx = in_group / (ni * nj), t = in_group - idx * (ni * nj);
+    const int tj = t / ni, ti = t - tj * ni;             // (the tiles that share rows of X^T are neighbours)
+    const int64_t xm = (int64_t)idx * g.sm * g.sn * CELL, slot = (int64_t)g.count * g.sm * g.sm * CELL;
+    Ring<TI, TJ, RING> ring;
+    constexpr int FI = TI / 2, FJ = TJ / 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave >> 1, wj = wave & 1;
+    const int64_t row_bytes = (int64_t)g.sm * CELL;
+    const char* xt = ws + g.xt[op.to ^ 1] + xm;
+    ring.run(lds, ws + g.s + op.r * slot + (int64_t)idx * g.sm * g.sm * CELL, xt, row_bytes, ti, tj, g.sm, g.sn, 0, g.sm, [&]() {
+        ring.clear();
+        ring.add(xt, row_bytes, ti * TI + wi * FI, tj * TJ + wj * FJ, g.sm, g.sn, op.scale_x);     // (the k loop reads it again, from cache)
+    });
+    const Sub sub = {reinterpret_cast<uint32_t(*)[33]>(lds + wave * 32 * 33 * 4)};
+    const int rows = g.trans ? g.n : g.m, cols = g.trans ? g.m : g.n, mat = g.first + idx;
+    const float rate = OUT == OUT_MUON ? io.lr * sqrtf(fmaxf(1.f, (float)rows / (float)cols)) : 0.f;
+    // four floats of a row of the caller's matrix a lane, where its rows allow it
+    float* param = OUT == OUT_MUON ? ptr.param[mat] : nullptr;
+    const bool wide = OUT == OUT_MUON && (cols & 3) == 0 && ((uintptr_t)param & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < FI; ++i) {
+        float4 old[FJ][4];
+        if constexpr (OUT == OUT_MUON) {                 // (the row's parameters at once: their latency is paid once)
+            if (wide) {
+#pragma unroll
+                for (int j = 0; j < FJ; ++j)
+#pragma unroll
+                    for (int it = 0; it < 4; ++it) {
+                        const int ci = ti * TI + wi * FI + i, cj = tj * TJ + wj * FJ + j;
+                        const int r = (g.trans ? cj : ci) * 32 + it * 8 + (lane >> 3), c = (g.trans ? ci : cj) * 32 + (lane & 7) * 4;
+                        old[j][it] = r < rows && c < cols ? *reinterpret_cast<const float4*>(param + (int64_t)r * cols + c)
+                                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) {
+            const int ci = ti * TI + wi * FI + i, cj = tj * TJ + wj * FJ + j;
+            if (ci >= g.sm || cj >= g.sn) continue;
+            put_acc<OUT == OUT_X>(sub, lane, ring.acc[i][j], op.out_scale * (OUT == OUT_X ? 1.f : 0x1p-15f));
+            if constexpr (OUT == OUT_X) {
+                sub.store<false>(ws + g.x + xm + ((int64_t)ci * g.sn + cj) * CELL, lane);
+                sub.store<true>(ws + g.xt[op.to] + xm + ((int64_t)cj * g.sm + ci) * CELL, lane);
+            } else {
+                const int r0 = (g.trans ? cj : ci) * 32, c0 = (g.trans ? ci : cj) * 32;
+                if (wide) {
+#pragma unroll
+                    for (int it = 0; it < 4; ++it) {
+                        const int r = it * 8 + (lane >> 3), c = (lane & 7) * 4;
+                        if (r0 + r >= rows || c0 + c >= cols) continue;
+                        float o[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = __builtin_bit_cast(float, g.trans ? sub.at[c + e][r] : sub.at[r][c + e]);
+                        float4 w = old[j][it];
+                        w.x = __builtin_fmaf(-rate, o[0], w.x * io.keep);
+                        w.y = __builtin_fmaf(-rate, o[1], w.y * io.keep);
+                        w.z = __builtin_fmaf(-rate, o[2], w.z * io.keep);
+                        w.w = __builtin_fmaf(-rate, o[3], w.w * io.keep);
+                        *reinterpret_cast<float4*>(param + (int64_t)(r0 + r) * cols + c0 + c) = w;
+                    }
+                    continue;
+                }
+#pragma unroll
+                for (int it = 0; it < 16; ++it) {
+                    const int r = it * 2 + (lane >> 5), c = lane & 31;
+                    if (r0 + r >= rows || c0 + c >= cols) continue;
+                    const float o = __builtin_bit_cast(float, g.trans ? sub.at[c][r] : sub.at[r][c]);
+                    if constexpr (OUT == OUT_MUON) {
+                        float* w = param + (int64_t)(r0 + r) * cols + c0 + c;
+                        *w = __builtin_fmaf(-rate, o, *w * io.keep);
+                    } else {
+                        const int64_t at = mat * io.out_matrix + (int64_t)(r0 + r) * io.out_row + c0 + c;
+                        if (OUT == OUT_F32) ((float*)io.out)[at] = o;
+                        else if (OUT == OUT_BF16) ((__bf16*)io.out)[at] = (__bf16)o;
+                        else ((_Float16*)io.out)[at] = (_Float16)o;
+                    }
+                }
+            }
+        }
+    }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------------
 inline int cells_of(int64_t n) { return (int)((n + 31) / 32); }
-
-// workspace: partial sums of the norms, then each group's X, X^T (two), S, R
-size_t layout(Plan& plan, int matrices) {
-    int64_t at = (int64_t)matrices * NORM_BLOCKS * sizeof(double);
-    for (int k = 0; k < plan.groups; ++k) {
-        Group& g = plan.g[k];
-        const int64_t x = (int64_t)g.count * g.sm * g.sn * CELL, s = (int64_t)g.count * g.sm * g.sm * CELL;
-        g.x = at;
-        g.xt[0] = at + x;
-        g.xt[1] = at + 2 * x;
-        g.s = at + 3 * x;
-        g.r = g.s + s;
-        at = g.r + s;
-    }
-    return (size_t)at;
-}
 
 Group group_of(int rows, int cols, int count, int first) {
     Group g = {};
@@ -427,50 +594,204 @@ Group group_of(int rows, int cols, int count, int first) {
     return g;
 }
 
-// first_tile of a launch with TI x TJ cells a workgroup; the number of workgroups, or -1 where they do not fit a grid
-int64_t count_tiles(Plan& plan, int t, bool sym) {
+// first_tile of a launch with t x tj cells a workgroup; the number of tiles
+int64_t count_tiles(Plan& plan, int t, int tj, bool sym) {
     int64_t total = 0;
     for (int k = 0; k < plan.groups; ++k) {
         const Group& g = plan.g[k];
-        const int64_t ni = (g.sm + t - 1) / t, nj = (g.sn + t - 1) / t;
-        plan.first_tile[k] = (int)total;
+        const int64_t ni = (g.sm + t - 1) / t, nj = (g.sn + tj - 1) / tj;
+        plan.first_tile[k] = total > 0x7fffffff ? 0x7fffffff : (int)total;
         total += g.count * (sym ? ni * (ni + 1) / 2 : ni * nj);
-        if (total > 0x7fffffff) return -1;
     }
-    plan.first_tile[plan.groups] = (int)total;
+    plan.first_tile[plan.groups] = total > 0x7fffffff ? 0x7fffffff : (int)total;
     return total;
 }
 
-template <int T, int WI, int WJ, int RING, int WHAT, int OUT>
-int launch_product(const Plan& plan, const Pointers& ptr, const Ends& io, int to, int64_t tiles, char* ws, hipStream_t stream) {
+constexpr int CUS = 256;
+
+// rows of cells of a workgroup in a launch of X's products
+int cut_mix(Plan& plan, int64_t& tiles) {
+    // 8 x 4 cells read each operand less often, where the k loop is long enough to carry their start and end
+    if ((tiles = count_tiles(plan, 8, 4, false)) >= 2 * CUS && plan.g[0].sm >= 64 && plan.groups == 1) return 8;
+    if ((tiles = count_tiles(plan, 4, 4, false)) >= CUS / 2) return 4;
+    tiles = count_tiles(plan, 2, 2, false);
+    return 2;
+}
+
+// T of a launch of symmetric products; sets the plan's workgroups and parts, and the floats that the parts' accumulators
+// take
+int cut_sym(Plan& plan, bool from_x, int64_t& workgroups, int64_t& floats) {
+    floats = 0;
+    int64_t work = 0, most = 0;
+    for (int k = 0; k < plan.groups; ++k) plan.parts[k] = 1;
+    const int64_t tiles = count_tiles(plan, 4, 4, true);
+    for (int k = 0; k < plan.groups; ++k) {
+        const Group& g = plan.g[k];
+        const int64_t n = (g.sm + 3) / 4, cells = from_x ? g.sn : g.sm;
+        work += g.count * (n * (n + 1) / 2) * cells;
+        most = cells > most ? cells : most;
+    }
+    // a workgroup's share of the k cells, if all shares were equal and two workgroups were on each CU; at least 16 cells,
+    // whose 16 K products a partial result's 64 KB out and in cost less than
+    int64_t share = (work + 2 * CUS - 1) / (2 * CUS);
+    if (share < 16) share = 16;
+    workgroups = tiles;
+    if (most >= share + share / 2) {
+        workgroups = 0;
+        for (int k = 0; k < plan.groups; ++k) {
+            const Group& g = plan.g[k];
+            const int64_t n = (g.sm + 3) / 4, cells = from_x ? g.sn : g.sm, count = g.count * (n * (n + 1) / 2);
+            const int64_t parts = cells >= share + share / 2 ? (cells + share - 1) / share : 1;
+            plan.parts[k] = (int)parts;
+            plan.first_tile[k] = workgroups > 0x7fffffff ? 0x7fffffff : (int)workgroups;
+            plan.partial[k] = floats;
+            workgroups += count * parts;
+            if (parts > 1) floats += 2 * count * parts * 16 * 1024;              // (two operations in a launch)
+        }
+        plan.first_tile[plan.groups] = workgroups > 0x7fffffff ? 0x7fffffff : (int)workgroups;
+        return 4;
+    }
+    if (tiles >= CUS / 2) return 4;
+    workgroups = count_tiles(plan, 2, 2, true);
+    return 2;
+}
+
+// Steps can go through the m x m side in blocks: S after a step is R S R with R = a I + B, and j steps are one product of X
+// with R .. R'.  A block of j steps takes (5 j - 4) m^3 instead of j m^3 flop in symmetric products and saves j - 1 passes
+// over X, 3 m^2 n flop each.  The price is digits: the identity part alpha = a^j of the block's product cancels most of the
+// largest singular values (their factor is near a^-j of it).  Frobenius errors measured against 64 bits, m >= 64, spectra
+// from flat to four decades: 1.3e-6 to 5.9e-6 step by step (fp32 products: 1.3e-6 to 5.1e-6), at most 1.2 times that with
+// two steps first, 2e-6 to 7.5e-6 with three and two.  So fp32 results get the first; 16-bit results, whose own rounding is
+// 2e-4 and more, and the Muon step, whose parameters keep 1e-7 of it, the second.  Below m = 64 (few rounding errors to
+// average) and where X is not wide, step by step.
+int next_block(const Plan& plan, bool exact, int done, int steps) {
+    double wide = 0, square = 0;
+    for (int k = 0; k < plan.groups; ++k) {
+        const Group& g = plan.g[k];
+        if (g.m < 64) return 1;
+        wide += (double)g.count * g.m * g.m * g.n;
+        square += (double)g.count * g.m * g.m * g.m;
+    }
+    if (wide < 1.25 * square) return 1;
+    const int most = done == 0 ? (exact ? 2 : 3) : done == 3 ? 2 : 1, left = steps - done;
+    return left < most ? left : most;
+}
+
+constexpr int SLOTS_ONE = 2, SLOTS_TWO = 4, SLOTS_THREE = 5;
+
+// workspace: partial sums of the norms, the partial accumulators of split products, then each group's X, X^T (two) and
+// slots
+size_t layout(Plan& plan, bool exact, int matrices, int64_t& partial) {
+    int64_t at = (int64_t)matrices * NORM_BLOCKS * sizeof(double);
+    partial = at;
+    int64_t most = 0;
+    for (int from_x = 0; from_x < 2; ++from_x) {
+        int64_t workgroups, floats;
+        cut_sym(plan, from_x, workgroups, floats);
+        most = floats > most ? floats : most;
+    }
+    at += most * sizeof(float);
+    const int block = next_block(plan, exact, 0, 3), slots = block == 3 ? SLOTS_THREE : block == 2 ? SLOTS_TWO : SLOTS_ONE;
+    for (int k = 0; k < plan.groups; ++k) {
+        Group& g = plan.g[k];
+        const int64_t x = (int64_t)g.count * g.sm * g.sn * CELL, s = (int64_t)g.count * g.sm * g.sm * CELL;
+        g.x = at;
+        g.xt[0] = at + x;
+        g.xt[1] = at + 2 * x;
+        g.s = at + 3 * x;
+        at = g.s + slots * s;
+    }
+    return (size_t)at;
+}
+
+struct Job {
+    Plan plan;
+    Pointers ptr;
+    Ends io;
+    int matrices, steps;
+    double eps;
+    char* ws;
+    int64_t partial;                     // offset of the partial accumulators
+    hipStream_t stream;
+};
+
+template <int T, int RING>
+int launch_sym(const Job& job, const SymOps& ops, int count, int64_t workgroups, bool parts) {
     constexpr size_t lds = (size_t)RING * T * 4 * PIECE;
     static unsigned long long done;
     if (lds > 64 * 1024) {
-        const int e = nf_raise_lds_cap((const void*)orth_product_kernel<T, T, WI, WJ, RING, WHAT, OUT>, &done);
+        const int e = nf_raise_lds_cap((const void*)orth_sym_kernel<T, RING>, &done);
         if (e) return e;
     }
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_product_kernel<T, T, WI, WJ, RING, WHAT, OUT>), dim3((unsigned)tiles),
-                       dim3(WI * WJ * 64), lds, stream, plan, ptr, io, to, ws);
+    float* partial = (float*)(job.ws + job.partial);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_sym_kernel<T, RING>), dim3((unsigned)workgroups, count), dim3(256), lds, job.stream,
+                       job.plan, ops, partial, job.ws);
+    const int e = nf_launch_status();
+    if (e || !parts) return e;
+    if constexpr (T == 4) {
+        Plan plan = job.plan;                            // the groups with parts, a wave a cell
+        int64_t total = 0;
+        int groups = 0;
+        for (int k = 0; k < job.plan.groups; ++k) {
+            if (job.plan.parts[k] == 1) continue;
+            const Group& g = plan.g[groups] = job.plan.g[k];
+            const int64_t n = (g.sm + 3) / 4;
+            plan.parts[groups] = job.plan.parts[k];
+            plan.partial[groups] = job.plan.partial[k];
+            plan.first_tile[groups++] = (int)total;
+            total += g.count * (n * (n + 1) / 2) * 4;
+            if (total > 0x1fffffff) return NF_ERR_SHAPE;
+        }
+        plan.groups = groups;
+        plan.first_tile[groups] = (int)total;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_sym_finish_kernel<T>), dim3((unsigned)total, count), dim3(256), 0, job.stream, plan,
+                           ops, partial, job.ws);
+        return nf_launch_status();
+    }
+    return NF_OK;
+}
+
+int sym(Job& job, const SymOps& ops, int count) {
+    int64_t workgroups, floats;
+    const int t = cut_sym(job.plan, ops.op[0].p == FROM_X, workgroups, floats);
+    if (workgroups > 0x7fffffff) return NF_ERR_SHAPE;
+    if (t == 4) return launch_sym<4, 4>(job, ops, count, workgroups, floats != 0);
+    return launch_sym<2, 4>(job, ops, count, workgroups, false);
+}
+
+int sym(Job& job, SymOp op) { return sym(job, SymOps{{op, op}}, 1); }
+
+template <int TI, int TJ, int RING, int OUT>
+int launch_mix(const Job& job, const MixOp& op, int64_t tiles) {
+    constexpr size_t lds = (size_t)RING * (TI + TJ) * 2 * PIECE;
+    static unsigned long long done;
+    if (lds > 64 * 1024) {
+        const int e = nf_raise_lds_cap((const void*)orth_mix_kernel<TI, TJ, RING, OUT>, &done);
+        if (e) return e;
+    }
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_mix_kernel<TI, TJ, RING, OUT>), dim3((unsigned)tiles), dim3(256), lds, job.stream, job.plan,
+                       job.ptr, job.io, op, job.ws);
     return nf_launch_status();
 }
 
-template <int WHAT, int OUT>
-int product(Plan& plan, const Pointers& ptr, const Ends& io, int to, char* ws, hipStream_t stream) {
-    // the largest tile that still gives most of the 256 CUs one
-    constexpr bool SYM = WHAT == MAKE_S || WHAT == MAKE_R;
-    int64_t tiles = count_tiles(plan, 8, SYM);
-    if (tiles >= 128) return launch_product<8, 2, 4, 4, WHAT, OUT>(plan, ptr, io, to, tiles, ws, stream);
-    tiles = count_tiles(plan, 4, SYM);
-    if (tiles >= 128) return launch_product<4, 2, 2, 3, WHAT, OUT>(plan, ptr, io, to, tiles, ws, stream);
-    tiles = count_tiles(plan, 2, SYM);
-    if (tiles < 0) return NF_ERR_SHAPE;
-    return launch_product<2, 2, 2, 4, WHAT, OUT>(plan, ptr, io, to, tiles, ws, stream);
+template <int OUT>
+int mix(Job& job, const MixOp& op) {
+    int64_t tiles;
+    const int t = cut_mix(job.plan, tiles);
+    if (tiles > 0x7fffffff) return NF_ERR_SHAPE;
+    if (t == 8) return launch_mix<8, 4, 3, OUT>(job, op, tiles);
+    if (t == 4) return launch_mix<4, 4, 4, OUT>(job, op, tiles);
+    return launch_mix<2, 2, 4, OUT>(job, op, tiles);
 }
 
+// Scales (powers of two) of the slots: S and M = R S 15 (|M| < 1.45), B = b S + c S S 14, and of alpha I + T, the product of
+// j steps' R, its T: 14 for one step (T = B), 11 for two (|T| <= a^2 = 11.9), 9 for three (40.9).
+#define TWO(e) ldexpf(1.f, e)
+
 template <typename T, bool MUON, int OUT>
-int run(Plan& plan, const Pointers& ptr, const Ends& io, int matrices, int steps, double eps, void* workspace, hipStream_t stream) {
-    char* ws = (char*)workspace;
-    double* partial = (double*)workspace;
+int run(Job& job) {
+    Plan& plan = job.plan;
+    double* partial = (double*)job.ws;
     int64_t most = 1;
     for (int k = 0; k < plan.groups; ++k) {
         const int64_t size = (int64_t)plan.g[k].m * plan.g[k].n;
@@ -478,8 +799,8 @@ int run(Plan& plan, const Pointers& ptr, const Ends& io, int matrices, int steps
     }
     int64_t blocks = (most + 4095) / 4096;
     if (blocks > NORM_BLOCKS) blocks = NORM_BLOCKS;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_norm_kernel<T, MUON>), dim3((unsigned)blocks, (unsigned)matrices), dim3(256), 0, stream,
-                       plan, ptr, io, partial);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_norm_kernel<T, MUON>), dim3((unsigned)blocks, (unsigned)job.matrices), dim3(256), 0,
+                       job.stream, plan, job.ptr, job.io, partial);
     int e = nf_launch_status();
     if (e) return e;
     int64_t total = 0;
@@ -488,16 +809,34 @@ int run(Plan& plan, const Pointers& ptr, const Ends& io, int matrices, int steps
         total += (int64_t)plan.g[k].count * (((int64_t)plan.g[k].sm * plan.g[k].sn + 3) / 4);
         if (total > 0x7fffffff) return NF_ERR_SHAPE;
     }
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_start_kernel<T, MUON>), dim3((unsigned)total), dim3(256), 0, stream, plan, ptr, io,
-                       partial, (int)blocks, eps, ws);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_start_kernel<T, MUON>), dim3((unsigned)total), dim3(256), 0, job.stream, plan, job.ptr,
+                       job.io, partial, (int)blocks, job.eps, job.ws);
     if ((e = nf_launch_status())) return e;
-    for (int s = 0; s < steps; ++s) {
-        const int to = (s + 1) & 1;
-        if ((e = product<MAKE_S, OUT_F32>(plan, ptr, io, to, ws, stream))) return e;
-        if ((e = product<MAKE_R, OUT_F32>(plan, ptr, io, to, ws, stream))) return e;
-        if (s + 1 < steps) e = product<MAKE_X, OUT_F32>(plan, ptr, io, to, ws, stream);
-        else e = product<MAKE_LAST, OUT>(plan, ptr, io, to, ws, stream);
-        if (e) return e;
+    const float a2 = CA * CA;
+    for (int s = 0, to = 1; s < job.steps; to ^= 1) {
+        const int block = next_block(plan, OUT == OUT_F32, s, job.steps);
+        MixOp op;
+        if ((e = sym(job, {FROM_X, FROM_X, 0, NONE, NONE, TWO(-15), 0.f, 0.f}))) return e;            // S = X X^T
+        if ((e = sym(job, {0, 0, 1, 0, NONE, CC * TWO(-16), CB / CC * TWO(15), 0.f}))) return e;            // B
+        if (block == 1) {
+            op = {1, to, CA * TWO(14), TWO(-14)};
+        } else {
+            if ((e = sym(job, {1, 0, 2, 0, NONE, TWO(-14), CA * TWO(14), 0.f}))) return e;                       // M = a S + B S
+            if ((e = sym(job, {1, 2, 3, 2, NONE, TWO(-14), CA * TWO(14), 0.f}))) return e;                       // S' = a M + B M
+            if ((e = sym(job, {3, 3, 0, 3, NONE, CC * TWO(-16), CB / CC * TWO(15), 0.f}))) return e;        // B'
+            const SymOps two = {{{0, 1, 2, 1, 0, TWO(-17), CA * TWO(14), CA * TWO(14)},                // T' = a B + a B' + B' B
+                                 {0, 3, 4, 3, NONE, TWO(-14), CA * TWO(14), 0.f}}};                              // M' = a S' + B' S'
+            if ((e = sym(job, two, block - 1))) return e;
+            op = {2, to, a2 * TWO(11), TWO(-11)};
+            if (block == 3) {
+                if ((e = sym(job, {0, 4, 1, 4, NONE, TWO(-14), CA * TWO(14), 0.f}))) return e;                   // S'' = a M' + B' M'
+                if ((e = sym(job, {1, 1, 3, 1, NONE, CC * TWO(-16), CB / CC * TWO(15), 0.f}))) return e;    // B''
+                if ((e = sym(job, {3, 2, 0, 2, 3, TWO(-16), CA * TWO(14), a2 * TWO(11)}))) return e;   // T'' = a T' + a^2 B'' + B'' T'
+                op = {0, to, a2 * CA * TWO(9), TWO(-9)};
+            }
+        }
+        s += block;
+        if ((e = s < job.steps ? mix<OUT_X>(job, op) : mix<OUT>(job, op))) return e;
     }
     return NF_OK;
 }
@@ -538,12 +877,13 @@ int plan_muon(const int* rows, const int* cols, int from, int count, Plan& plan,
 
 }  // namespace
 
-extern "C" size_t nf_orthogonalize_workspace_bytes(int64_t count, int rows, int cols) {
-    if (!sizes_ok(count, rows, cols) || count == 0) return 0;
+extern "C" size_t nf_orthogonalize_workspace_bytes(int64_t count, int rows, int cols, int elem) {
+    if (!nf_elem_size(elem) || !sizes_ok(count, rows, cols) || count == 0) return 0;
     Plan plan = {};
     plan.groups = 1;
     plan.g[0] = group_of(rows, cols, (int)count, 0);
-    return layout(plan, (int)count);
+    int64_t partial;
+    return layout(plan, elem == NF_ELEM_F32, (int)count, partial);
 }
 
 extern "C" int nf_orthogonalize(const void* matrices, int64_t matrix_stride, int64_t row_stride, void* out,
@@ -558,22 +898,24 @@ extern "C" int nf_orthogonalize(const void* matrices, int64_t matrix_stride, int
         (count > 1 && out_matrix_stride < (rows - 1) * out_row_stride + cols) || !nf_aligned(matrices, size) ||
         !nf_aligned(out, size) || !nf_aligned(workspace, 16))
         return NF_ERR_LAYOUT;
-    Plan plan = {};
-    plan.groups = 1;
-    plan.g[0] = group_of(rows, cols, (int)count, 0);
-    if (workspace_bytes < layout(plan, (int)count)) return NF_ERR_SCRATCH;
-    Pointers ptr = {};
-    Ends io = {};
-    io.in = matrices;
-    io.out = out;
-    io.in_matrix = matrix_stride;
-    io.in_row = row_stride;
-    io.out_matrix = out_matrix_stride;
-    io.out_row = out_row_stride;
-    hipStream_t s = (hipStream_t)stream;
-    if (elem == NF_ELEM_F32) return run<float, false, OUT_F32>(plan, ptr, io, (int)count, steps, eps, workspace, s);
-    if (elem == NF_ELEM_BF16) return run<__bf16, false, OUT_BF16>(plan, ptr, io, (int)count, steps, eps, workspace, s);
-    return run<_Float16, false, OUT_F16>(plan, ptr, io, (int)count, steps, eps, workspace, s);
+    Job job = {};
+    job.plan.groups = 1;
+    job.plan.g[0] = group_of(rows, cols, (int)count, 0);
+    if (workspace_bytes < layout(job.plan, elem == NF_ELEM_F32, (int)count, job.partial)) return NF_ERR_SCRATCH;
+    job.io.in = matrices;
+    job.io.out = out;
+    job.io.in_matrix = matrix_stride;
+    job.io.in_row = row_stride;
+    job.io.out_matrix = out_matrix_stride;
+    job.io.out_row = out_row_stride;
+    job.matrices = (int)count;
+    job.steps = steps;
+    job.eps = eps;
+    job.ws = (char*)workspace;
+    job.stream = (hipStream_t)stream;
+    if (elem == NF_ELEM_F32) return run<float, false, OUT_F32>(job);
+    if (elem == NF_ELEM_BF16) return run<__bf16, false, OUT_BF16>(job);
+    return run<_Float16, false, OUT_F16>(job);
 }
 
 extern "C" size_t nf_muon_workspace_bytes(const int* rows, const int* cols, int count) {
@@ -585,7 +927,8 @@ extern "C" size_t nf_muon_workspace_bytes(const int* rows, const int* cols, int 
             if (!sizes_ok(1, rows[i], cols[i])) return 0;
         Plan plan = {};
         const int taken = plan_muon(rows, cols, at, count, plan, order);
-        const size_t need = layout(plan, taken);
+        int64_t partial;
+        const size_t need = layout(plan, false, taken, partial);
         most = need > most ? need : most;
         at += taken;
     }
@@ -607,21 +950,24 @@ extern "C" int nf_muon_update(float* const* params, const float* const* grads, f
     if (workspace_bytes < nf_muon_workspace_bytes(rows, cols, count)) return NF_ERR_SCRATCH;
     int order[MAX_MATRICES];
     for (int at = 0; at < count;) {
-        Plan plan = {};
-        const int taken = plan_muon(rows, cols, at, count, plan, order);
-        layout(plan, taken);
-        Pointers ptr = {};
+        Job job = {};
+        const int taken = plan_muon(rows, cols, at, count, job.plan, order);
+        layout(job.plan, false, taken, job.partial);
         for (int i = 0; i < taken; ++i) {
-            ptr.grad[i] = grads[order[i]];
-            ptr.momentum[i] = momenta[order[i]];
-            ptr.param[i] = params[order[i]];
+            job.ptr.grad[i] = grads[order[i]];
+            job.ptr.momentum[i] = momenta[order[i]];
+            job.ptr.param[i] = params[order[i]];
         }
-        Ends io = {};
-        io.momentum = (float)momentum;
-        io.nesterov = nesterov;
-        io.keep = (float)(1.0 - lr * weight_decay);
-        io.lr = (float)lr;
-        const int e = run<float, true, OUT_MUON>(plan, ptr, io, taken, steps, eps, workspace, (hipStream_t)stream);
+        job.io.momentum = (float)momentum;
+        job.io.nesterov = nesterov;
+        job.io.keep = (float)(1.0 - lr * weight_decay);
+        job.io.lr = (float)lr;
+        job.matrices = taken;
+        job.steps = steps;
+        job.eps = eps;
+        job.ws = (char*)workspace;
+        job.stream = (hipStream_t)stream;
+        const int e = run<float, true, OUT_MUON>(job);
         if (e) return e;
         at += taken;
     }

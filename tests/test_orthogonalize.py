@@ -104,11 +104,12 @@ def test_refusals():
 def test_argument_errors_before_launch():
     lib = nf._lib.load()
     one = 1 << 12                                       # (a non-NULL pointer that nothing reads: every call is refused)
-    need = lib.nf_orthogonalize_workspace_bytes(2, 33, 70)
+    need = lib.nf_orthogonalize_workspace_bytes(2, 33, 70, 0)
     # norms; X and twice X^T of 2 x 3 cells, S and R of 2 x 2 cells, 4 KB each
     assert need == 2 * 256 * 8 + 2 * (3 * 6 + 2 * 4) * 4096
-    assert lib.nf_orthogonalize_workspace_bytes(0, 3, 3) == 0
-    assert lib.nf_orthogonalize_workspace_bytes(1, 0, 3) == 0 and lib.nf_orthogonalize_workspace_bytes(1, 3, 2 ** 20 + 1) == 0
+    assert lib.nf_orthogonalize_workspace_bytes(0, 3, 3, 0) == 0
+    assert lib.nf_orthogonalize_workspace_bytes(1, 0, 3, 0) == 0 and lib.nf_orthogonalize_workspace_bytes(1, 3, 2 ** 20 + 1, 0) == 0
+    assert lib.nf_orthogonalize_workspace_bytes(1, 3, 3, 3) == 0
 
     def call(g=one, ms=33 * 70, rs=70, out=one, oms=33 * 70, ors=70, ws=one, nbytes=need, count=2, rows=33, cols=70, steps=5,
              eps=1e-7, elem=0):
@@ -204,7 +205,7 @@ def test_strides(kind):
 def test_a_batch_is_cut_where_its_workspace_ends(monkeypatch):
     g = gradients((7, 40, 33), 6)
     want = nf.orthogonalize(g)
-    monkeypatch.setattr(nf._lib, 'WORKSPACE_BYTES', 3 * nf._lib.load().nf_orthogonalize_workspace_bytes(1, 40, 33))
+    monkeypatch.setattr(nf._lib, 'WORKSPACE_BYTES', 3 * nf._lib.load().nf_orthogonalize_workspace_bytes(1, 40, 33, 0))
     assert torch.equal(nf.orthogonalize(g), want)
     monkeypatch.setattr(nf._lib, 'WORKSPACE_BYTES', 1)
     assert torch.equal(nf.orthogonalize(g), want)
