@@ -30,6 +30,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+constexpr double DA = 3.4445, DB = -4.7750, DC = 2.0315;
 constexpr float CA = 3.4445f, CB = -4.7750f, CC = 2.0315f;
 constexpr int CELL = 4096;               // bytes of a 32 x 32 cell
 constexpr int PIECE = 1024;              // of one term of one 32 x 16 block
@@ -114,9 +115,19 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(Plan plan, Pointers ptr,
 }
 
 // ---- cells ---------------------------------------------------------------------------------------------------------------
-// a value as its two terms: hi in the low half, lo in the high half of a word
+// A value's two terms.  The empty asm makes v one rounded number: where it is a product, the compiler may otherwise round
+// the exact product to hi in one place and v in another, and where these differ (once in some 2^13 values) hi + lo is off by
+// a step of hi.
+__device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
+    asm("" : "+v"(v));
+    hi = (_Float16)v;
+    lo = (_Float16)(v - (float)hi);
+}
+
+// both in a word, hi in the low half
 __device__ __forceinline__ uint32_t split(float v) {
-    const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
+    _Float16 hi, lo;
+    split(v, hi, lo);
     return (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
 }
 
@@ -203,12 +214,14 @@ __device__ __forceinline__ void piece_to_lds(const char* src, unsigned dst) {
 }
 
 // A symmetric result in slot `out`: k0 (P Q^T + k1 E1 + k2 E2), the factors with the powers of two of the operands' scales
-// (P = Q = X where p is FROM_X, else slots; E1, E2: slots or NONE).  The E's are where the accumulators start from.
+// (P = Q = X where p is FROM_X, else slots; E1, E2: slots or NONE).  The E's join the accumulators when the product is
+// complete: an accumulator that started from them would round every one of its 3 K / 16 sums at their size (measured: twice
+// the error of the whole iteration).
 constexpr int FROM_X = -1, NONE = -1;
 struct SymOp { int p, q, out, e1, e2; float k0, k1, k2; };
 struct SymOps { SymOp op[2]; };
-// X <- alpha X + T X from slot r: the accumulators start from scale_x * X (alpha with T's power of two), and out_scale takes
-// them back to X's scale
+// X <- alpha X + T X from slot r: the accumulators get scale_x * X (alpha with T's power of two), and out_scale takes them
+// back to X's scale
 struct MixOp { int r, to; float scale_x, out_scale; };
 
 // vmcnt(N) lgkmcnt(0): at most N loads on their way, all LDS reads back
@@ -290,8 +303,10 @@ struct Ring {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
     }
-    // acc += scale * E, from the cells of E^T (rows as Q's, columns as P's): an accumulator's four rows are 8 bytes there
-    __device__ __forceinline__ void add(const char* et, int64_t row_bytes, int ci0, int cj0, int prows, int qrows, float scale) {
+    // E of this wave's cells in the accumulators' layout, from the cells of E^T (rows as Q's, columns as P's): an
+    // accumulator's four rows are 8 bytes there
+    struct Terms { f16x4 v[FI][FJ][4][2]; };
+    __device__ __forceinline__ void load(Terms& t, const char* et, int64_t row_bytes, int ci0, int cj0, int prows, int qrows) const {
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int i = 0; i < FI; ++i)
@@ -299,25 +314,29 @@ struct Ring {
             for (int j = 0; j < FJ; ++j) {
                 const int ci = ci0 + i < prows ? ci0 + i : prows - 1, cj = cj0 + j < qrows ? cj0 + j : qrows - 1;
                 const char* cell = et + cj * row_bytes + (int64_t)ci * CELL + (lane & 31) * 16 + (lane >> 5) * 8;
-                f16x4 hi[4], lo[4];
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {            // rows 8 g + 4 (lane / 32) .. + 3
-                    const char* at = cell + (g >> 1) * 2 * PIECE + (g & 1) * 512;
-                    hi[g] = *reinterpret_cast<const f16x4*>(at);
-                    lo[g] = *reinterpret_cast<const f16x4*>(at + PIECE);
-                }
+                for (int g = 0; g < 4; ++g)              // rows 8 g + 4 (lane / 32) .. + 3
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        t.v[i][j][g][h] = *reinterpret_cast<const f16x4*>(cell + (g >> 1) * 2 * PIECE + (g & 1) * 512 + h * PIECE);
+            }
+    }
+    __device__ __forceinline__ void add(const Terms& t, float scale) {
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+            for (int j = 0; j < FJ; ++j)
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        acc[i][j][4 * g + e] = __builtin_fmaf(scale, (float)hi[g][e] + (float)lo[g][e], acc[i][j][4 * g + e]);
-                if (FI * FJ > 4) __builtin_amdgcn_sched_barrier(0);      // (all cells' loads at once would not fit the registers)
-            }
+                        acc[i][j][4 * g + e] = __builtin_fmaf(scale, (float)t.v[i][j][g][0][e] + (float)t.v[i][j][g][1][e], acc[i][j][4 * g + e]);
     }
-    // k cells first .. last - 1 (at least one); `start` sets the accumulators while the first blocks are on their way
-    template <typename Start>
+    // k cells first .. last - 1 (at least one); `ahead` is called where all blocks have been requested, for what the epilogue
+    // wants to have by then
+    template <typename Ahead>
     __device__ __forceinline__ void run(char* lds, const char* p, const char* q, int64_t row_bytes, int ti, int tj, int prows,
-                                        int qrows, int first, int last, Start start) {
+                                        int qrows, int first, int last, Ahead ahead) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wi = wave >> 1, wj = wave & 1;
         const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
@@ -337,7 +356,7 @@ struct Ring {
 #pragma unroll
         for (int s = 0; s < RING; ++s)
             if (s < steps) fill();
-        start();
+        clear();
         if (steps > RING) meet<(RING - 1) * LOADS>();
         else meet<0>();
 #pragma unroll
@@ -357,6 +376,7 @@ struct Ring {
             step<1, false, true>();
             s += 2;
         }
+        ahead();
         for (; s + 2 < steps; s += 2) {                  // the last blocks are all requested
             meet<0>();
             step<0, false, true>();
@@ -423,11 +443,16 @@ __global__ __launch_bounds__(256) void orth_sym_kernel(Plan plan, SymOps ops, fl
     constexpr int F = T / 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave >> 1, wj = wave & 1;
     const int64_t row_bytes = (int64_t)kcells * CELL;
+    typename Ring<T, T, RING>::Terms e;
+    const bool has_e1 = op.e1 != NONE && part == 0, has_e2 = op.e2 != NONE && part == 0;
     ring.run(lds, p, q, row_bytes, ti, tj, g.sm, g.sm, first, last, [&]() {
-        ring.clear();
-        if (op.e1 != NONE && part == 0) ring.add(slots + op.e1 * slot, row_bytes, ti * T + wi * F, tj * T + wj * F, g.sm, g.sm, op.k1);
-        if (op.e2 != NONE && part == 0) ring.add(slots + op.e2 * slot, row_bytes, ti * T + wi * F, tj * T + wj * F, g.sm, g.sm, op.k2);
+        if (has_e1) ring.load(e, slots + op.e1 * slot, row_bytes, ti * T + wi * F, tj * T + wj * F, g.sm, g.sm);
     });
+    if (has_e1) ring.add(e, op.k1);
+    if (has_e2) {
+        ring.load(e, slots + op.e2 * slot, row_bytes, ti * T + wi * F, tj * T + wj * F, g.sm, g.sm);
+        ring.add(e, op.k2);
+    }
     const Sub sub = {reinterpret_cast<uint32_t(*)[33]>(lds + wave * 32 * 33 * 4)};
 #pragma unroll
     for (int i = 0; i < F; ++i)
@@ -506,10 +531,14 @@ __global__ __launch_bounds__(256, 2) void orth_mix_kernel(Plan plan, Pointers pt
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave >> 1, wj = wave & 1;
     const int64_t row_bytes = (int64_t)g.sm * CELL;
     const char* xt = ws + g.xt[op.to ^ 1] + xm;
+    // X's own part from the rows of X^T that were Q's, from cache; with many cells a wave, only when the fragments are done
+    typename Ring<TI, TJ, RING>::Terms e;
+    auto own = [&]() { ring.load(e, xt, row_bytes, ti * TI + wi * FI, tj * TJ + wj * FJ, g.sm, g.sn); };
     ring.run(lds, ws + g.s + op.r * slot + (int64_t)idx * g.sm * g.sm * CELL, xt, row_bytes, ti, tj, g.sm, g.sn, 0, g.sm, [&]() {
-        ring.clear();
-        ring.add(xt, row_bytes, ti * TI + wi * FI, tj * TJ + wj * FJ, g.sm, g.sn, op.scale_x);     // (the k loop reads it again, from cache)
+        if (FI * FJ <= 4) own();
     });
+    if (FI * FJ > 4) own();
+    ring.add(e, op.scale_x);
     const Sub sub = {reinterpret_cast<uint32_t(*)[33]>(lds + wave * 32 * 33 * 4)};
     const int rows = g.trans ? g.n : g.m, cols = g.trans ? g.m : g.n, mat = g.first + idx;
     const float rate = OUT == OUT_MUON ? io.lr * sqrtf(fmaxf(1.f, (float)rows / (float)cols)) : 0.f;
@@ -576,6 +605,362 @@ __global__ __launch_bounds__(256, 2) void orth_mix_kernel(Plan plan, Pointers pt
                 }
             }
         }
+    }
+}
+
+// ---- matrices with a side of at most 32 --------------------------------------------------------------------------------------
+// All of the iteration is a polynomial of S = G G^T applied to G, and S is 32 x 32: two passes over G (S; the product with
+// the polynomial) instead of three per step, everything in fp64 on its matrix instructions, whose 16 digits the recursion
+// S <- R S R, Q <- R Q (R = a + b S + c S S) cannot spend.  The norm is the trace of S.  A workgroup takes a part of the
+// columns; where there is more than one, a first launch leaves the partial sums of S and a second one adds them, iterates (in
+// every workgroup alike, 18 products of 32 x 32: 7 us) and applies.  Measured 64 us -> 12 us for 16 x 2048 against the
+// general path.
+constexpr int TINY = 32, TINY_K = 128;
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// D = P Q of 32 x 32, Q symmetric: a wave has the 16 x 16 tile (wave / 2, wave % 2), row lane / 16 + 4 r, column lane % 16
+__device__ __forceinline__ f64x4 tiny_product(const double (*p)[33], const double (*q)[33], int ti, int tj, int lane) {
+    f64x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < 32; k += 4)
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64(p[16 * ti + (lane & 15)][k + (lane >> 4)], q[16 * tj + (lane & 15)][k + (lane >> 4)],
+                                                   acc, 0, 0, 0);
+    return acc;
+}
+
+enum { TINY_SUM, TINY_APPLY, TINY_BOTH };
+
+template <typename T, bool MUON>
+__global__ __launch_bounds__(256) void orth_tiny_kernel(Plan plan, Pointers ptr, Ends io, int what, int steps, double eps,
+                                                        double* __restrict__ partial) {
+    __shared__ float x[32][TINY_K + 4];
+    __shared__ double s[32][33], q[32][33], r[32][33], m[32][33];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ti = wave >> 1, tj = wave & 1;
+    int k = 0;
+    while (k + 1 < plan.groups && (int)blockIdx.x >= plan.first_tile[k + 1]) ++k;
+    const Group& g = plan.g[k];
+    const int parts = plan.parts[k], in_group = blockIdx.x - plan.first_tile[k], idx = in_group / parts, part = in_group - idx * parts;
+    const int mat = g.first + idx, cols = g.trans ? g.m : g.n;
+    const int each = ((g.n + parts - 1) / parts + TINY_K - 1) / TINY_K * TINY_K;
+    const int first = part * each, last = first + each < g.n ? first + each : g.n;
+    const T* in = MUON ? nullptr : (const T*)io.in + mat * io.in_matrix;
+    const float* gr = MUON ? ptr.grad[mat] : nullptr;
+    float* mo = MUON ? ptr.momentum[mat] : nullptr;
+    // columns c0 .. c0 + 127 of X (a row of the caller's matrix side by side in a wave); `update`: the momentum's step
+    auto stage = [&](int c0, bool update) {
+        __syncthreads();
+        constexpr int EACH = 32 * TINY_K / 256;
+        float v[EACH], gv[EACH];
+#pragma unroll
+        for (int l = 0; l < EACH; ++l) {                 // (all loads before the first use: their latency is paid once)
+            const int e = threadIdx.x + 256 * l, i = g.trans ? e & 31 : e / TINY_K, c = g.trans ? e >> 5 : e % TINY_K;
+            const bool in_range = i < g.m && c0 + c < last;
+            const int row = in_range ? (g.trans ? c0 + c : i) : 0, col = in_range ? (g.trans ? i : c0 + c) : 0;
+            if constexpr (MUON) {
+                v[l] = mo[(int64_t)row * cols + col];
+                gv[l] = gr[(int64_t)row * cols + col];
+            } else {
+                v[l] = (float)in[(int64_t)row * io.in_row + col];
+            }
+        }
+#pragma unroll
+        for (int l = 0; l < EACH; ++l) {
+            const int e = threadIdx.x + 256 * l, i = g.trans ? e & 31 : e / TINY_K, c = g.trans ? e >> 5 : e % TINY_K;
+            const bool in_range = i < g.m && c0 + c < last;
+            if constexpr (MUON) {
+                if (update) {
+                    v[l] = __builtin_fmaf(io.momentum, v[l], gv[l]);
+                    if (in_range) mo[(int64_t)(g.trans ? c0 + c : i) * cols + (g.trans ? i : c0 + c)] = v[l];
+                }
+                if (io.nesterov) v[l] = __builtin_fmaf(io.momentum, v[l], gv[l]);
+            }
+            x[i][c] = in_range ? v[l] : 0.f;
+        }
+        __syncthreads();
+    };
+    double* sums = partial + plan.partial[k] + (int64_t)idx * parts * (TINY * TINY);
+    if (what != TINY_APPLY) {
+        f64x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        for (int c0 = first; c0 < last; c0 += TINY_K) {
+            stage(c0, true);
+#pragma unroll 8
+            for (int c = 0; c < TINY_K; c += 4)
+                acc[c >> 2 & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)x[16 * ti + (lane & 15)][c + (lane >> 4)],
+                                                                       (double)x[16 * tj + (lane & 15)][c + (lane >> 4)],
+                                                                       acc[c >> 2 & 1], 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * ti + (lane >> 4) + 4 * e, col = 16 * tj + (lane & 15);
+            if (what == TINY_SUM) sums[part * (TINY * TINY) + row * TINY + col] = acc[0][e] + acc[1][e];
+            else s[row][col] = acc[0][e] + acc[1][e];
+        }
+        if (what == TINY_SUM) return;
+    } else {
+        for (int e = threadIdx.x; e < TINY * TINY; e += 256) {
+            double v = 0;
+            for (int p = 0; p < parts; ++p) v += sums[p * (TINY * TINY) + e];
+            s[e >> 5][e & 31] = v;
+        }
+    }
+    __syncthreads();
+    double trace = 0;
+    for (int i = 0; i < TINY; ++i) trace += s[i][i];
+    const double scale = 1.0 / (sqrt(trace) + eps);
+    __syncthreads();
+    for (int e = threadIdx.x; e < TINY * TINY; e += 256) {
+        s[e >> 5][e & 31] *= scale * scale;
+        q[e >> 5][e & 31] = (e >> 5) == (e & 31);
+    }
+    __syncthreads();
+    for (int step = 0; step < steps; ++step) {
+        const f64x4 ss = tiny_product(s, s, ti, tj, lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * ti + (lane >> 4) + 4 * e, col = 16 * tj + (lane & 15);
+            r[row][col] = (row == col ? DA : 0.0) + DB * s[row][col] + DC * ss[e];
+        }
+        __syncthreads();
+        const f64x4 rq = tiny_product(r, q, ti, tj, lane), rs = tiny_product(r, s, ti, tj, lane);
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * ti + (lane >> 4) + 4 * e, col = 16 * tj + (lane & 15);
+            q[row][col] = rq[e];
+            m[row][col] = rs[e];
+        }
+        __syncthreads();
+        if (step + 1 < steps) {
+            const f64x4 sn = tiny_product(r, m, ti, tj, lane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[16 * ti + (lane >> 4) + 4 * e][16 * tj + (lane & 15)] = sn[e];
+            __syncthreads();
+        }
+    }
+    const float rate = MUON ? io.lr * sqrtf(fmaxf(1.f, g.trans ? (float)g.n / (float)g.m : (float)g.m / (float)g.n)) : 0.f;
+    for (int c0 = first; c0 < last; c0 += TINY_K) {
+        if (what == TINY_APPLY || last - first > TINY_K) stage(c0, false);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {                    // a wave's columns: 32 of the 128, both row tiles
+            const int ri = t & 1, cj = wave * 2 + (t >> 1);
+            f64x4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < 32; c += 4)
+                acc = __builtin_amdgcn_mfma_f64_16x16x4f64(q[16 * ri + (lane & 15)][c + (lane >> 4)],
+                                                           (double)x[c + (lane >> 4)][16 * cj + (lane & 15)], acc, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 16 * ri + (lane >> 4) + 4 * e, j = c0 + 16 * cj + (lane & 15);
+                if (i >= g.m || j >= last) continue;
+                const float o = (float)(acc[e] * scale);
+                const int row = g.trans ? j : i, col = g.trans ? i : j;
+                if constexpr (MUON) {
+                    float* w = ptr.param[mat] + (int64_t)row * cols + col;
+                    *w = __builtin_fmaf(-rate, o, *w * io.keep);
+                } else {
+                    ((T*)io.out)[mat * io.out_matrix + (int64_t)row * io.out_row + col] = (T)o;
+                }
+            }
+        }
+    }
+}
+
+// ---- matrices that fit one workgroup's LDS ------------------------------------------------------------------------------------
+// Sides of 33 to 96 whose X, X^T and S fit it (2 SM SN + SM SM cells of 4 KB; 64 x 256 and 96 x 128 at most): one launch for
+// everything, a workgroup of eight waves per matrix with up to NC cells of X a wave.  The products are those of the general
+// path, step by step.
+constexpr int SMALL_CELLS = 38;          // 152 KB
+
+__device__ __forceinline__ f16x8 fragment(const char* cell, int h, int term, int lane) {
+    return *reinterpret_cast<const f16x8*>(cell + (2 * h + term) * PIECE + lane * 16);
+}
+
+// acc += P Q^T of one cell pair's k block: the cross terms in an accumulator of their own (two chains instead of one)
+__device__ __forceinline__ void terms(f32x16& acc, f32x16& cross, f16x8 a0, f16x8 a1, f16x8 b0, f16x8 b1) {
+    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b1, cross, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b0, acc, 0, 0, 0);
+    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, b0, cross, 0, 0, 0);
+}
+
+// acc += scale * (the cell whose transpose is `cell`): an accumulator's four rows are 8 bytes there
+__device__ __forceinline__ void add_from(f32x16& acc, const char* cell, int lane, float scale) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const char* at = cell + (g >> 1) * 2 * PIECE + (g & 1) * 512 + (lane & 31) * 16 + (lane >> 5) * 8;
+        const f16x4 hi = *reinterpret_cast<const f16x4*>(at), lo = *reinterpret_cast<const f16x4*>(at + PIECE);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[4 * g + e] = __builtin_fmaf(scale, (float)hi[e] + (float)lo[e], acc[4 * g + e]);
+    }
+}
+
+// the sum over `cells` k cells of one cell's product
+__device__ __forceinline__ f32x16 cell_product(const char* p, const char* q, int cells, int lane) {
+    f32x16 acc, cross;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = cross[r] = 0.f;
+#pragma unroll 2
+    for (int k = 0; k < cells; ++k, p += CELL, q += CELL)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            terms(acc, cross, fragment(p, h, 0, lane), fragment(p, h, 1, lane), fragment(q, h, 0, lane), fragment(q, h, 1, lane));
+    return acc + cross;
+}
+
+// scale * acc to its cell and to the transposed one.  A cell on the diagonal is its own transpose and is written once: of two
+// entries that differ in their last bit, hi of one and lo of the other are a third value.
+__device__ __forceinline__ void store_both(char* cell, char* transposed, const f32x16& acc, float scale, int lane) {
+    char* mine = cell + ((lane >> 4) & 1) * 2 * PIECE + ((lane >> 3) & 1) * 512 + (lane & 7) * 2;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        f16x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            _Float16 h, l;
+            split(scale * acc[4 * g + e], h, l);
+            hi[e] = h;
+            lo[e] = l;
+            if (cell != transposed) {
+                char* at = mine + (8 * g + 4 * (lane >> 5) + e) * 16;
+                *reinterpret_cast<_Float16*>(at) = h;
+                *reinterpret_cast<_Float16*>(at + PIECE) = l;
+            }
+        }
+        char* at = transposed + (g >> 1) * 2 * PIECE + (g & 1) * 512 + (lane & 31) * 16 + (lane >> 5) * 8;
+        *reinterpret_cast<f16x4*>(at) = hi;
+        *reinterpret_cast<f16x4*>(at + PIECE) = lo;
+    }
+}
+
+template <int SM, int NC, typename T, bool MUON>
+__global__ __launch_bounds__(512) void orth_small_kernel(Group g, Pointers ptr, Ends io, int steps, double eps) {
+    constexpr int SYM = (SM * (SM + 1) / 2 + 7) / 8;     // cells i <= j of S a wave
+    extern __shared__ __align__(16) char lds[];
+    __shared__ double red[8];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cells = SM * g.sn, mat = g.first + blockIdx.x;
+    char *x = lds, *xt = lds + cells * CELL, *s = lds + 2 * cells * CELL;
+    const int rows = g.trans ? g.n : g.m, cols = g.trans ? g.m : g.n;
+    const T* in = MUON ? nullptr : (const T*)io.in + mat * io.in_matrix;
+    const float* gr = MUON ? ptr.grad[mat] : nullptr;
+    float* mo = MUON ? ptr.momentum[mat] : nullptr;
+    {
+        float v[NC][16], gv[NC][16];
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+            const int c = t * 8 + wave, cj = c / SM, ci = c - cj * SM;
+#pragma unroll
+            for (int it = 0; it < 16; ++it) {
+                const int r = (g.trans ? cj : ci) * 32 + it * 2 + (lane >> 5), col = (g.trans ? ci : cj) * 32 + (lane & 31);
+                const bool in_range = c < cells && r < rows && col < cols;
+                if constexpr (MUON) {
+                    v[t][it] = in_range ? mo[(int64_t)r * cols + col] : 0.f;
+                    gv[t][it] = in_range ? gr[(int64_t)r * cols + col] : 0.f;
+                } else {
+                    v[t][it] = in_range ? (float)in[(int64_t)r * io.in_row + col] : 0.f;
+                }
+            }
+        }
+        double sum = 0;
+#pragma unroll
+        for (int t = 0; t < NC; ++t)
+#pragma unroll
+            for (int it = 0; it < 16; ++it) {
+                if constexpr (MUON) {
+                    const int c = t * 8 + wave, cj = c / SM, ci = c - cj * SM;
+                    const int r = (g.trans ? cj : ci) * 32 + it * 2 + (lane >> 5), col = (g.trans ? ci : cj) * 32 + (lane & 31);
+                    v[t][it] = __builtin_fmaf(io.momentum, v[t][it], gv[t][it]);
+                    if (c < cells && r < rows && col < cols) mo[(int64_t)r * cols + col] = v[t][it];
+                    if (io.nesterov) v[t][it] = __builtin_fmaf(io.momentum, v[t][it], gv[t][it]);
+                }
+                sum += (double)v[t][it] * v[t][it];
+            }
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        if (lane == 0) red[wave] = sum;
+        __syncthreads();
+        sum = 0;
+        for (int w = 0; w < 8; ++w) sum += red[w];
+        const double scale = 32768.0 / (sqrt(sum) + eps);
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+            const int c = t * 8 + wave, cj = c / SM, ci = c - cj * SM;
+            if (c >= cells) continue;
+#pragma unroll
+            for (int it = 0; it < 16; ++it) {
+                _Float16 hi, lo;
+                split((float)((double)v[t][it] * scale), hi, lo);
+                const int a = it * 2 + (lane >> 5), b = lane & 31, r = g.trans ? b : a, k = g.trans ? a : b;    // in X's cell
+                char* to = x + (ci * g.sn + cj) * CELL + (k >> 4) * 2 * PIECE + (r + 32 * ((k >> 3) & 1)) * 16 + (k & 7) * 2;
+                *reinterpret_cast<_Float16*>(to) = hi;
+                *reinterpret_cast<_Float16*>(to + PIECE) = lo;
+                to = xt + (cj * SM + ci) * CELL + (r >> 4) * 2 * PIECE + (k + 32 * ((r >> 3) & 1)) * 16 + (r & 7) * 2;
+                *reinterpret_cast<_Float16*>(to) = hi;
+                *reinterpret_cast<_Float16*>(to + PIECE) = lo;
+            }
+        }
+    }
+    __syncthreads();
+    // the symmetric cells of this wave
+    int si[SYM], sj[SYM];
+#pragma unroll
+    for (int u = 0; u < SYM; ++u) {
+        int p = u * 8 + wave, i = 0;
+        while (i < SM && p >= SM - i) p -= SM - i++;
+        si[u] = i;                                       // (SM: none)
+        sj[u] = i + p;
+    }
+    const float rate = MUON ? io.lr * sqrtf(fmaxf(1.f, (float)rows / (float)cols)) : 0.f;
+    for (int step = 0; step < steps; ++step) {
+        f32x16 sa[SYM], xa[NC];
+#pragma unroll
+        for (int u = 0; u < SYM; ++u) {
+            if (si[u] >= SM) continue;
+            sa[u] = cell_product(x + si[u] * g.sn * CELL, x + sj[u] * g.sn * CELL, g.sn, lane);
+            store_both(s + (si[u] * SM + sj[u]) * CELL, s + (sj[u] * SM + si[u]) * CELL, sa[u], 0x1p-15f, lane);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < SYM; ++u) {
+            if (si[u] >= SM) continue;
+            sa[u] = cell_product(s + si[u] * SM * CELL, s + sj[u] * SM * CELL, SM, lane);
+            add_from(sa[u], s + (sj[u] * SM + si[u]) * CELL, lane, CB / CC * 0x1p15f);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < SYM; ++u)
+            if (si[u] < SM)
+                store_both(s + (si[u] * SM + sj[u]) * CELL, s + (sj[u] * SM + si[u]) * CELL, sa[u], CC * 0x1p-16f, lane);
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+            const int c = t * 8 + wave, cj = c / SM, ci = c - cj * SM;
+            if (c >= cells) continue;
+            xa[t] = cell_product(s + ci * SM * CELL, xt + cj * SM * CELL, SM, lane);
+            add_from(xa[t], xt + (cj * SM + ci) * CELL, lane, CA * 0x1p14f);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+            const int c = t * 8 + wave, cj = c / SM, ci = c - cj * SM;
+            if (c >= cells) continue;
+            if (step + 1 < steps) {
+                store_both(x + (ci * g.sn + cj) * CELL, xt + (cj * SM + ci) * CELL, xa[t], 0x1p-14f, lane);
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int i = ci * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), j = cj * 32 + (lane & 31);
+                if (i >= g.m || j >= g.n) continue;
+                const int r = g.trans ? j : i, col = g.trans ? i : j;
+                const float o = xa[t][e] * 0x1p-29f;
+                if constexpr (MUON) {
+                    float* w = ptr.param[mat] + (int64_t)r * cols + col;
+                    *w = __builtin_fmaf(-rate, o, *w * io.keep);
+                } else {
+                    ((T*)io.out)[mat * io.out_matrix + (int64_t)r * io.out_row + col] = (T)o;
+                }
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -651,7 +1036,8 @@ int cut_sym(Plan& plan, bool from_x, int64_t& workgroups, int64_t& floats) {
         plan.first_tile[plan.groups] = workgroups > 0x7fffffff ? 0x7fffffff : (int)workgroups;
         return 4;
     }
-    if (tiles >= CUS / 2) return 4;
+    // short k loops (up to 512) leave a large tile's start and end uncovered: four small ones on its CU overlap them
+    if (tiles >= CUS / 2 && most > 16) return 4;
     workgroups = count_tiles(plan, 2, 2, true);
     return 2;
 }
@@ -679,9 +1065,35 @@ int next_block(const Plan& plan, bool exact, int done, int steps) {
 
 constexpr int SLOTS_ONE = 2, SLOTS_TWO = 4, SLOTS_THREE = 5;
 
-// workspace: partial sums of the norms, the partial accumulators of split products, then each group's X, X^T (two) and
+// the tiny groups' workgroups and parts; the doubles of their partial sums (0: one launch does it all)
+int64_t cut_tiny(Plan& plan) {
+    int64_t total = 0, doubles = 0;
+    bool any = false;
+    for (int k = 0; k < plan.groups; ++k) {
+        const Group& g = plan.g[k];
+        // (two rounds of one workgroup cost what a launch more does; past 64 parts adding them would)
+        int64_t each = g.n <= 2 * TINY_K ? g.n : TINY_K;
+        if ((g.n + each - 1) / each > 64) each = (g.n + 64 * TINY_K - 1) / (64 * TINY_K) * TINY_K;
+        const int64_t parts = (g.n + each - 1) / each;
+        plan.parts[k] = (int)parts;
+        plan.partial[k] = doubles;
+        plan.first_tile[k] = total > 0x7fffffff ? 0x7fffffff : (int)total;
+        total += g.count * parts;
+        any = any || parts > 1;
+        doubles += g.count * parts * (TINY * TINY);
+    }
+    plan.first_tile[plan.groups] = total > 0x7fffffff ? 0x7fffffff : (int)total;
+    return any ? doubles : 0;
+}
+
+// workspace: the tiny groups' partial sums (they are done with before the rest begins); over them partial sums of the norms, the partial accumulators of split products, then each group's X, X^T (two) and
 // slots
-size_t layout(Plan& plan, bool exact, int matrices, int64_t& partial) {
+// (the small ones need none)
+size_t layout(Plan& plan, Plan& tiny, bool exact, int64_t& partial) {
+    const size_t doubles = (size_t)cut_tiny(tiny) * sizeof(double), least = doubles > 16 ? doubles : 16;
+    if (!plan.groups) return least;
+    const Group& end = plan.g[plan.groups - 1];
+    const int matrices = end.first + end.count;
     int64_t at = (int64_t)matrices * NORM_BLOCKS * sizeof(double);
     partial = at;
     int64_t most = 0;
@@ -701,14 +1113,14 @@ size_t layout(Plan& plan, bool exact, int matrices, int64_t& partial) {
         g.s = at + 3 * x;
         at = g.s + slots * s;
     }
-    return (size_t)at;
+    return (size_t)at > least ? (size_t)at : least;
 }
 
 struct Job {
-    Plan plan;
+    Plan plan, small, tiny;              // the groups by the path they take
     Pointers ptr;
     Ends io;
-    int matrices, steps;
+    int steps;
     double eps;
     char* ws;
     int64_t partial;                     // offset of the partial accumulators
@@ -788,9 +1200,70 @@ int mix(Job& job, const MixOp& op) {
 // j steps' R, its T: 14 for one step (T = B), 11 for two (|T| <= a^2 = 11.9), 9 for three (40.9).
 #define TWO(e) ldexpf(1.f, e)
 
+template <typename T, bool MUON>
+int run_tiny(const Job& job) {
+    const Plan& plan = job.tiny;
+    bool parts = false;
+    for (int k = 0; k < plan.groups; ++k) parts = parts || plan.parts[k] > 1;
+    for (int what = parts ? TINY_SUM : TINY_BOTH; what <= (parts ? TINY_APPLY : TINY_BOTH); ++what) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_tiny_kernel<T, MUON>), dim3((unsigned)plan.first_tile[plan.groups]), dim3(256), 0,
+                           job.stream, plan, job.ptr, job.io, what, job.steps, job.eps, (double*)job.ws);
+        const int e = nf_launch_status();
+        if (e) return e;
+    }
+    return NF_OK;
+}
+
+// (nf_raise_lds_cap leaves no room for this kernel's static LDS)
+int raise_lds(const void* kernel, unsigned long long* done) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return (int)e;
+    const unsigned long long bit = (dev >= 0 && dev < 64) ? 1ull << dev : 0ull;
+    if (bit && (__atomic_load_n(done, __ATOMIC_ACQUIRE) & bit)) return NF_OK;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_CELLS * CELL);
+    if (e != hipSuccess) return (int)e;
+    if (bit) __atomic_fetch_or(done, bit, __ATOMIC_RELEASE);
+    return NF_OK;
+}
+
+template <int SM, int NC, typename T, bool MUON>
+int launch_small(const Job& job, const Group& g) {
+    static unsigned long long done;
+    const int e = raise_lds((const void*)orth_small_kernel<SM, NC, T, MUON>, &done);
+    if (e) return e;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_small_kernel<SM, NC, T, MUON>), dim3(g.count), dim3(512), SM * (2 * g.sn + SM) * CELL, job.stream, g,
+                       job.ptr, job.io, job.steps, job.eps);
+    return nf_launch_status();
+}
+
+template <typename T, bool MUON>
+int run_small(const Job& job) {
+    for (int k = 0; k < job.small.groups; ++k) {
+        const Group& g = job.small.g[k];
+        const int nc = (g.sm * g.sn + 7) / 8;
+        int e = NF_ERR_SHAPE;
+        if (g.sm == 2) e = nc == 1 ? launch_small<2, 1, T, MUON>(job, g) : launch_small<2, 2, T, MUON>(job, g);
+        else if (g.sm == 3) e = launch_small<3, 2, T, MUON>(job, g);
+        if (e) return e;
+    }
+    return NF_OK;
+}
+
 template <typename T, bool MUON, int OUT>
 int run(Job& job) {
     Plan& plan = job.plan;
+    if (job.small.groups) {
+        const int e = run_small<T, MUON>(job);
+        if (e) return e;
+    }
+    if (job.tiny.groups) {
+        if (job.tiny.first_tile[job.tiny.groups] == 0x7fffffff) return NF_ERR_SHAPE;
+        const int e = run_tiny<T, MUON>(job);
+        if (e) return e;
+    }
+    if (!plan.groups) return NF_OK;
+    const int matrices = plan.g[plan.groups - 1].first + plan.g[plan.groups - 1].count;
     double* partial = (double*)job.ws;
     int64_t most = 1;
     for (int k = 0; k < plan.groups; ++k) {
@@ -799,7 +1272,7 @@ int run(Job& job) {
     }
     int64_t blocks = (most + 4095) / 4096;
     if (blocks > NORM_BLOCKS) blocks = NORM_BLOCKS;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_norm_kernel<T, MUON>), dim3((unsigned)blocks, (unsigned)job.matrices), dim3(256), 0,
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_norm_kernel<T, MUON>), dim3((unsigned)blocks, (unsigned)matrices), dim3(256), 0,
                        job.stream, plan, job.ptr, job.io, partial);
     int e = nf_launch_status();
     if (e) return e;
@@ -848,9 +1321,17 @@ bool sizes_ok(int64_t count, int rows, int cols) {
     return count >= 0 && count <= MAX_MATRIX_GRID && rows >= 1 && cols >= 1 && rows <= MAX_SIDE && cols <= MAX_SIDE;
 }
 
+// 0: the general path, 1: one workgroup's LDS, 2: tiny
+int path_of(const int* shape) {
+    const int sm = cells_of(shape[0] < shape[1] ? shape[0] : shape[1]), sn = cells_of(shape[0] < shape[1] ? shape[1] : shape[0]);
+    return sm == 1 ? 2 : sm <= 3 && sm * (2 * sn + sm) <= SMALL_CELLS ? 1 : 0;
+}
+Plan& plan_of(Job& job, int path) { return path == 0 ? job.plan : path == 1 ? job.small : job.tiny; }
+int longer(const int* shape) { return shape[0] > shape[1] ? shape[0] : shape[1]; }
+
 // The matrices from `from` on that one sequence of launches takes, grouped by shape: `order` lists them group by group.
 // Returns how many.
-int plan_muon(const int* rows, const int* cols, int from, int count, Plan& plan, int* order) {
+int plan_muon(const int* rows, const int* cols, int from, int count, Job& job, int* order) {
     int taken = 0, shapes[MAX_GROUPS][2], groups = 0, of[MAX_MATRICES];
     while (from + taken < count && taken < MAX_MATRICES) {
         const int r = rows[from + taken], c = cols[from + taken];
@@ -864,26 +1345,47 @@ int plan_muon(const int* rows, const int* cols, int from, int count, Plan& plan,
         }
         of[taken++] = k;
     }
-    int at = 0;
-    plan.groups = groups;
+    // where the general path runs anyway, what it does for matrices of 64 and more rows costs no launch of their own
+    int path[MAX_GROUPS];
+    bool general = false;
+    for (int k = 0; k < groups; ++k) general = (path[k] = path_of(shapes[k])) == 0 || general;
+    for (int k = 0; k < groups; ++k)
+        if (general && path[k] == 1 && shapes[k][0] >= 64 && shapes[k][1] >= 64) path[k] = 0;
+    // by path; the widest first: their workgroups run longest
+    int at = 0, rank[MAX_GROUPS];
     for (int k = 0; k < groups; ++k) {
-        const int first = at;
+        int j = k;
+        for (; j > 0; --j) {
+            const int o = rank[j - 1];
+            if (path[k] != path[o] ? path[k] > path[o] : longer(shapes[k]) <= longer(shapes[o])) break;
+            rank[j] = o;
+        }
+        rank[j] = k;
+    }
+    for (int k = 0; k < groups; ++k) {
+        const int first = at, shape = rank[k];
         for (int i = 0; i < taken; ++i)
-            if (of[i] == k) order[at++] = from + i;
-        plan.g[k] = group_of(shapes[k][0], shapes[k][1], at - first, first);
+            if (of[i] == shape) order[at++] = from + i;
+        Plan& to = plan_of(job, path[shape]);
+        to.g[to.groups++] = group_of(shapes[shape][0], shapes[shape][1], at - first, first);
     }
     return taken;
+}
+
+void plan_one(Job& job, int64_t count, int rows, int cols) {
+    const int shape[2] = {rows, cols};
+    Plan& to = plan_of(job, path_of(shape));
+    to.groups = 1;
+    to.g[0] = group_of(rows, cols, (int)count, 0);
 }
 
 }  // namespace
 
 extern "C" size_t nf_orthogonalize_workspace_bytes(int64_t count, int rows, int cols, int elem) {
     if (!nf_elem_size(elem) || !sizes_ok(count, rows, cols) || count == 0) return 0;
-    Plan plan = {};
-    plan.groups = 1;
-    plan.g[0] = group_of(rows, cols, (int)count, 0);
-    int64_t partial;
-    return layout(plan, elem == NF_ELEM_F32, (int)count, partial);
+    Job job = {};
+    plan_one(job, count, rows, cols);
+    return layout(job.plan, job.tiny, elem == NF_ELEM_F32, job.partial);
 }
 
 extern "C" int nf_orthogonalize(const void* matrices, int64_t matrix_stride, int64_t row_stride, void* out,
@@ -899,16 +1401,14 @@ extern "C" int nf_orthogonalize(const void* matrices, int64_t matrix_stride, int
         !nf_aligned(out, size) || !nf_aligned(workspace, 16))
         return NF_ERR_LAYOUT;
     Job job = {};
-    job.plan.groups = 1;
-    job.plan.g[0] = group_of(rows, cols, (int)count, 0);
-    if (workspace_bytes < layout(job.plan, elem == NF_ELEM_F32, (int)count, job.partial)) return NF_ERR_SCRATCH;
+    plan_one(job, count, rows, cols);
+    if (workspace_bytes < layout(job.plan, job.tiny, elem == NF_ELEM_F32, job.partial)) return NF_ERR_SCRATCH;
     job.io.in = matrices;
     job.io.out = out;
     job.io.in_matrix = matrix_stride;
     job.io.in_row = row_stride;
     job.io.out_matrix = out_matrix_stride;
     job.io.out_row = out_row_stride;
-    job.matrices = (int)count;
     job.steps = steps;
     job.eps = eps;
     job.ws = (char*)workspace;
@@ -925,10 +1425,9 @@ extern "C" size_t nf_muon_workspace_bytes(const int* rows, const int* cols, int 
     for (int at = 0; at < count;) {
         for (int i = at; i < count && i < at + MAX_MATRICES; ++i)
             if (!sizes_ok(1, rows[i], cols[i])) return 0;
-        Plan plan = {};
-        const int taken = plan_muon(rows, cols, at, count, plan, order);
-        int64_t partial;
-        const size_t need = layout(plan, false, taken, partial);
+        Job job = {};
+        const int taken = plan_muon(rows, cols, at, count, job, order);
+        const size_t need = layout(job.plan, job.tiny, false, job.partial);
         most = need > most ? need : most;
         at += taken;
     }
@@ -951,8 +1450,8 @@ extern "C" int nf_muon_update(float* const* params, const float* const* grads, f
     int order[MAX_MATRICES];
     for (int at = 0; at < count;) {
         Job job = {};
-        const int taken = plan_muon(rows, cols, at, count, job.plan, order);
-        layout(job.plan, false, taken, job.partial);
+        const int taken = plan_muon(rows, cols, at, count, job, order);
+        layout(job.plan, job.tiny, false, job.partial);
         for (int i = 0; i < taken; ++i) {
             job.ptr.grad[i] = grads[order[i]];
             job.ptr.momentum[i] = momenta[order[i]];
@@ -962,7 +1461,6 @@ extern "C" int nf_muon_update(float* const* params, const float* const* grads, f
         job.io.nesterov = nesterov;
         job.io.keep = (float)(1.0 - lr * weight_decay);
         job.io.lr = (float)lr;
-        job.matrices = taken;
         job.steps = steps;
         job.eps = eps;
         job.ws = (char*)workspace;
