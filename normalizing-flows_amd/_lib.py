@@ -23,6 +23,7 @@ NF_ERR_BINS = -4
 NF_ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 _lib = None
+_nodes = None
 
 _c = ctypes
 _SIGNATURES = {
@@ -283,6 +284,22 @@ def load():
     return _lib
 
 
+def nodes():
+    """The autograd nodes in C++ (csrc/nf_torch.cpp) over the loaded library.  Raises if absent."""
+    global _nodes
+    if _nodes is None:
+        lib = load()
+        try:
+            from . import _nf_torch
+        except ImportError as e:
+            raise RuntimeError('_nf_torch.so does not load (%s): build it with `python -c "import __graft_entry__ as g; '
+                               'g.build()"` (or `make -C normalizing-flows_amd/csrc`).  There is no fallback path.' % e)
+        _nf_torch.bind(*(_c.cast(getattr(lib, name), _c.c_void_p).value for name in
+                         ('nf_layer_norm_fwd', 'nf_layer_norm_bwd_workspace_bytes', 'nf_layer_norm_bwd', 'nf_strerror')))
+        _nodes = _nf_torch
+    return _nodes
+
+
 class NfError(RuntimeError):
     def __init__(self, code, where):
         self.code = code
@@ -311,14 +328,6 @@ def _rows(t, name):
     if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
         raise RuntimeError('%s must be 2-D with contiguous rows' % name)
     return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0)))
-
-
-def unit_rows(t):
-    """A 2-D tensor as the entry points take it: t itself, or a copy where its last axis is not contiguous (an expanded
-    gradient, a transposed view; contiguous() leaves the strides of an empty tensor as they are)."""
-    if t.shape[1] == 1 or t.stride(1) == 1:
-        return t
-    return t.contiguous() if t.numel() else t.new_empty(t.shape)
 
 
 def _stream():
@@ -1526,55 +1535,6 @@ def affine_bwd(x, params, layout, grad_y, grad_lad, inverse=False, feat_index=No
         _check(lib.nf_affine_bwd(xp, xs, _ptr(feat_index), pp, ps, int(layout), gyp, gys, _ptr(gl), gxp, gxs, gpp, gps,
                                  B, D, int(inverse), _stream()), 'nf_affine_bwd')
     return gx, gparams
-
-
-# ------------------------------------------------------------------------------------------------ layer normalisation
-def _norm_vector(t, name, features, device):
-    if t is None:
-        return None
-    _dev(t, name)
-    if t.dim() != 1 or t.shape[0] != features or t.device != device:
-        raise ValueError('%s must be a vector of %d elements on %s' % (name, features, device))
-    return t.detach().contiguous()
-
-
-def layer_norm(x, weight=None, bias=None, eps=1e-5, want_stats=False):
-    """Layer normalisation of the rows of x [rows, features] (fp32, bf16 or fp16; weight / bias fp32 or None):
-    (y, mean, rstd), the latter two fp32 [rows] and None unless want_stats."""
-    lib = load()
-    xp, xs = _rows(x, 'x')
-    rows, n = int(x.shape[0]), int(x.shape[1])
-    weight, bias = _norm_vector(weight, 'weight', n, x.device), _norm_vector(bias, 'bias', n, x.device)
-    y = torch.empty(rows, n, dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if want_stats:
-        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        _check(lib.nf_layer_norm_fwd(xp, xs, _ptr(weight), _ptr(bias), y.data_ptr(), n, _ptr(mean), _ptr(rstd), rows, n,
-                                     eps, NF_ELEM[x.dtype], _stream()), 'nf_layer_norm_fwd')
-    return y, mean, rstd
-
-
-def layer_norm_bwd(grad_y, x, mean, rstd, weight=None, want_x=True, want_weight=True, want_bias=True):
-    """(grad_x, grad_weight, grad_bias) of layer_norm from grad_y and what its forward pass kept; None for those not
-    wanted."""
-    lib = load()
-    gp, gs = _rows(grad_y, 'grad_y')
-    xp, xs = _rows(x, 'x')
-    rows, n = int(x.shape[0]), int(x.shape[1])
-    if grad_y.shape != x.shape or grad_y.dtype != x.dtype:
-        raise ValueError('grad_y must have the shape and type of x')
-    weight = _norm_vector(weight, 'weight', n, x.device)
-    elem = NF_ELEM[x.dtype]
-    gx = torch.empty(rows, n, dtype=x.dtype, device=x.device) if want_x else None
-    gw = torch.empty(n, dtype=torch.float32, device=x.device) if want_weight else None
-    gb = torch.empty(n, dtype=torch.float32, device=x.device) if want_bias else None
-    nbytes = lib.nf_layer_norm_bwd_workspace_bytes(rows, n, elem) if want_weight or want_bias else 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    with torch.cuda.device(x.device):
-        _check(lib.nf_layer_norm_bwd(gp, gs, xp, xs, mean.data_ptr(), rstd.data_ptr(), _ptr(weight), _ptr(gx), n, _ptr(gw),
-                                     _ptr(gb), _ptr(ws), nbytes, rows, n, elem, _stream()), 'nf_layer_norm_bwd')
-    return gx, gw, gb
 
 
 # ------------------------------------------------------------------------------------------------ matrix updates

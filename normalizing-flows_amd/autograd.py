@@ -19,8 +19,6 @@ model.py:233-244).  Here every forward kernel has a hand-written backward kernel
                    nf_rqs_bwd_max + the final layer's two GEMMs - in bf16 mode with the parameter gradients as a bf16
                    plane between the three kernels (nf_rqs_bwd_max_bf16, nf_masked_linear_split_bwd_input_bf16,
                    nf_masked_linear_half_bwd_weight_bf16)
-  LayerNormFn    : y = layer_norm(x; weight, bias) over rows; backward nf_layer_norm_bwd (input gradient and the weight /
-                   bias sums in one pass over x and grad_y)
 """
 import torch
 
@@ -382,20 +380,3 @@ class AffineFn(torch.autograd.Function):
         gx, gparams = _lib.affine_bwd(x, params, layout, grad_y.contiguous(), grad_lad, inverse=inverse,
                                       feat_index=feat_index, num_features=num_features)
         return gx, gparams, None, None, None, None
-
-
-class LayerNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _lib.layer_norm(x, weight, bias, eps, want_stats=True)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_y):
-        x, weight, mean, rstd = ctx.saved_tensors
-        grad_y = _lib.unit_rows(grad_y)
-        want = ctx.needs_input_grad
-        return (*_lib.layer_norm_bwd(grad_y, x, mean, rstd, weight, want_x=want[0], want_weight=want[1],
-                                     want_bias=want[2]), None)

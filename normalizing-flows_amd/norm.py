@@ -6,8 +6,6 @@ works on each sample alone.  Its statistics run over the hidden units, so it bel
 (``ResidualNet(use_layer_norm=True)``) and not between the masked layers of a MADE, where a unit would see the units of
 higher degree.
 """
-import numbers
-
 import torch
 from torch import nn
 
@@ -18,23 +16,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (biased variance; statistics in fp32).
 
     x: [..., features] on the GPU, float32, bfloat16 or float16, rows at any stride; the result has its shape and type.
-    weight, bias: float32 vectors of `features` elements, or None.  Differentiable once in x, weight and bias; the
-    gradients of weight and bias are summed in a fixed order (the same inputs give the same bits)."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise RuntimeError('x must be a tensor on the GPU (MI355X); this package has no CPU path')
-    if x.dtype not in _lib.NF_ELEM:
-        raise TypeError('x must be float32, bfloat16 or float16, got %s' % x.dtype)
-    if x.dim() < 1 or not 1 <= x.shape[-1] < 2 ** 31:
-        raise ValueError('x must have a last axis of at least one element, got shape %s' % (tuple(x.shape),))
-    if not isinstance(eps, numbers.Real) or not 0 <= eps < float('inf'):
-        raise ValueError('eps must be a finite number >= 0, got %r' % (eps,))
-    rows = _lib.unit_rows(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
-    if torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in (weight, bias))):
-        from .autograd import LayerNormFn
-        y = LayerNormFn.apply(rows, weight, bias, float(eps))
-    else:
-        y = _lib.layer_norm(rows, weight, bias, float(eps))[0]
-    return y.view(x.shape)
+    weight, bias: float32 vectors of `features` elements, or None.  Differentiable once (not under create_graph) in x, weight
+    and bias; the gradients of weight and bias are summed in a fixed order (the same inputs give the same bits)."""
+    return _lib.nodes().layer_norm(x, weight, bias, eps)
 
 
 class LayerNorm(nn.Module):

@@ -171,18 +171,22 @@ def test_empty_and_selected_gradients():
     xd.requires_grad_()
     (gx,) = torch.autograd.grad(nf.layer_norm(xd, wc.cuda()), (xd,), g.cuda())   # no sums
     close(gx, *bounds(x, wc, None, g, torch.float32)[1], 'grad_x alone')
-    y = nf.layer_norm(xd, wd)
-    (gx,) = torch.autograd.grad(y, (xd,), g.cuda().requires_grad_(), create_graph=True)
-    with pytest.raises(RuntimeError):
-        gx.sum().backward()                             # no second derivative
+    bd = torch.zeros(40, device='cuda', requires_grad=True)
+    (gb,) = torch.autograd.grad(nf.layer_norm(xd, None, bd), (bd,), g.cuda())    # a bias without a weight
+    close(gb, *bounds(x, None, bd.detach().cpu(), g, torch.float32)[3], 'grad_b alone')
+    with pytest.raises(RuntimeError, match='once'):     # no second derivative
+        torch.autograd.grad(nf.layer_norm(xd, wd), (xd,), g.cuda(), create_graph=True)
 
 
 @pytest.mark.gpu
 def test_refusals_on_the_device():
     x = torch.zeros(3, 4, device='cuda')
     for bad in (dict(weight=torch.ones(5, device='cuda')), dict(bias=torch.ones(3, device='cuda')), dict(eps=-1.0),
-                dict(eps=float('nan')), dict(eps='1')):
+                dict(eps=float('nan')), dict(eps=float('inf'))):
         with pytest.raises(ValueError):
+            nf.layer_norm(x, **bad)
+    for bad in (dict(eps='1'), dict(weight=1.0)):
+        with pytest.raises(TypeError):
             nf.layer_norm(x, **bad)
     with pytest.raises(TypeError):
         nf.layer_norm(x.double())
