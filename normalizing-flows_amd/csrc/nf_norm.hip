@@ -19,8 +19,7 @@ namespace {
 
 constexpr int EMAX = 32;                 // elements of a row that a thread keeps, in workgroups up to 256 threads
 constexpr int EMAX_WIDE = 16;            // in larger ones, whose threads have at most 128 registers
-constexpr int FWD_GRID = 2048;           // workgroups of the forward pass: eight per CU
-constexpr int BWD_GRID = 512;            // of the backward pass: each leaves a partial sum of 2 N floats
+constexpr int BWD_GRID = 1024;           // workgroups of the backward pass: each leaves a partial sum of 2 N floats
 constexpr int LONG_SLICES = 64;          // row slices of the long rows' weight gradient
 
 // 16 bytes of elements at the element's own alignment (global memory takes unaligned 16-byte accesses: odd row strides
@@ -33,18 +32,24 @@ template <typename T> struct Chunk {
 };
 
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T* p, int left, float* v) {
+__device__ __forceinline__ u32x4 load_raw(const T* p, int left) {
     constexpr int V = Chunk<T>::V;
-    if (left >= V) {
-        const u32x4 raw = *reinterpret_cast<const u32x4_at2*>(p);
-        const typename Chunk<T>::Elems e = __builtin_bit_cast(typename Chunk<T>::Elems, raw);
+    if (left >= V) return *reinterpret_cast<const u32x4_at2*>(p);
+    typename Chunk<T>::Elems e;
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = (float)e[k];
-    } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = k < left ? (float)p[k] : 0.f;
-    }
+    for (int k = 0; k < V; ++k) e[k] = k < left ? p[k] : (T)0.f;
+    return __builtin_bit_cast(u32x4, e);
 }
+
+template <typename T>
+__device__ __forceinline__ void widen(u32x4 raw, float* v) {
+    const typename Chunk<T>::Elems e = __builtin_bit_cast(typename Chunk<T>::Elems, raw);
+#pragma unroll
+    for (int k = 0; k < Chunk<T>::V; ++k) v[k] = (float)e[k];
+}
+
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T* p, int left, float* v) { widen<T>(load_raw(p, left), v); }
 
 template <typename T>
 __device__ __forceinline__ void store_chunk(T* p, int left, const float* v) {
@@ -61,20 +66,55 @@ __device__ __forceinline__ void store_chunk(T* p, int left, const float* v) {
     }
 }
 
-// Sum over the `tpr` threads of a row; every one of them gets it.  `red`: one float per wave; rows of several waves
-// must be summed by all threads of the workgroup together.
-__device__ __forceinline__ float row_sum(float v, int tpr, float* red) {
-    for (int o = (tpr < 64 ? tpr : 64) >> 1; o; o >>= 1) v += __shfl_xor(v, o);
-    if (tpr > 64) {
-        const int wave = threadIdx.x >> 6, per = tpr >> 6, first = wave & ~(per - 1);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[wave] = v;
-        __syncthreads();
-        v = 0.f;
-        for (int k = 0; k < per; ++k) v += red[first + k];
-    }
+template <int CTRL>
+__device__ __forceinline__ float add_lane(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+
+// sum over the lanes of a row within the wave (a part of it for tpr < 64): neighbours within 16 lanes by DPP
+__device__ __forceinline__ float lane_sum(float v, int tpr) {
+    if (tpr >= 2) v = add_lane<0xB1>(v);                 // lane ^ 1
+    if (tpr >= 4) v = add_lane<0x4E>(v);                 // lane ^ 2
+    if (tpr >= 8) v = add_lane<0x141>(v);                // the other four of eight, mirrored
+    if (tpr >= 16) v = add_lane<0x140>(v);               // the other eight of sixteen
+    if (tpr >= 32) v += __shfl_xor(v, 16);
+    if (tpr >= 64) v += __shfl_xor(v, 32);
     return v;
 }
+
+// Sums over the `tpr` threads of a row; every one of them gets them.  Rows of several waves must be summed by all threads of
+// the workgroup together, through `red`: two floats per wave, twice, taken in turn (`turn`), so that one barrier does.
+struct RowSum {
+    float (*red)[16][2];
+    int tpr, turn;
+    template <int N> __device__ __forceinline__ void sums(float (&v)[N]) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = lane_sum(v[k], tpr);
+        if (tpr <= 64) return;
+        const int wave = threadIdx.x >> 6, per = tpr >> 6, first = wave & ~(per - 1);
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < N; ++k) red[turn][wave][k] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = 0.f;
+        for (int w = first; w < first + per; ++w)
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] += red[turn][w][k];
+    }
+    __device__ __forceinline__ float sum(float a) {
+        float v[1] = {a};
+        sums(v);
+        return v[0];
+    }
+    __device__ __forceinline__ void sum(float& a, float& b) {
+        float v[2] = {a, b};
+        sums(v);
+        a = v[0];
+        b = v[1];
+    }
+};
 
 template <typename T, int C, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void norm_fwd_kernel(const T* __restrict__ x, int64_t xs, const float* __restrict__ w,
@@ -82,7 +122,8 @@ __global__ __launch_bounds__(BLOCK) void norm_fwd_kernel(const T* __restrict__ x
                                                         float* __restrict__ mean, float* __restrict__ rstd, int64_t rows,
                                                         int n, float eps, int tpr) {
     constexpr int V = Chunk<T>::V;
-    __shared__ float red[16];
+    __shared__ float red[2][16][2];
+    RowSum row_sum = {red, tpr, 0};
     const int t = threadIdx.x & (tpr - 1), per = blockDim.x / tpr;
     const float nf = (float)n;
     float wv[C][V], bv[C][V];
@@ -90,33 +131,38 @@ __global__ __launch_bounds__(BLOCK) void norm_fwd_kernel(const T* __restrict__ x
     for (int c = 0; c < C; ++c) {
         const int col = (c * tpr + t) * V;
 #pragma unroll
-        for (int e = 0; e < V; ++e) { wv[c][e] = 1.f; bv[c][e] = 0.f; }
-        if (col < n) {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (col + e < n) {
-                    if (w) wv[c][e] = w[col + e];
-                    if (b) bv[c][e] = b[col + e];
-                }
+        for (int e = 0; e < V; ++e) {
+            wv[c][e] = (w && col + e < n) ? w[col + e] : 1.f;
+            bv[c][e] = (b && col + e < n) ? b[col + e] : 0.f;
         }
     }
-    // (the same trip count for every thread of the workgroup: row_sum has barriers)
-    for (int64_t base = (int64_t)blockIdx.x * per; base < rows; base += (int64_t)gridDim.x * per) {
-        const int64_t row = base + threadIdx.x / tpr;
-        const bool live = row < rows;
-        const T* xr = x + (live ? row : 0) * xs;
-        float v[C][V], s = 0.f;
+    // the next row is requested while this one is summed where one workgroup fills a CU; smaller ones cover each other, and
+    // its registers would cost them more (131072 x 2048 bf16: 236 us without, 278 with)
+    constexpr bool AHEAD = BLOCK == 1024;
+    u32x4 ahead[C];
+    auto fetch = [&](int64_t row) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int col = (c * tpr + t) * V;
-            if (live && col < n) load_chunk(xr + col, n - col, v[c]);
-            else
+            if (row < rows && col < n) ahead[c] = load_raw(x + row * xs + col, n - col);
+            else ahead[c] = u32x4{0, 0, 0, 0};
+        }
+    };
+    // (the same trip count for every thread of the workgroup: sums of several waves have a barrier)
+    const int64_t stride = (int64_t)gridDim.x * per;
+    int64_t row = (int64_t)blockIdx.x * per + threadIdx.x / tpr;
+    if (AHEAD) fetch(row);
+    for (int64_t base = (int64_t)blockIdx.x * per; base < rows; base += stride, row += stride) {
+        float v[C][V], s = 0.f;
+        if (!AHEAD) fetch(row);
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[c][e] = 0.f;
+        for (int c = 0; c < C; ++c) {
+            widen<T>(ahead[c], v[c]);
 #pragma unroll
             for (int e = 0; e < V; ++e) s += v[c][e];
         }
-        const float mu = row_sum(s, tpr, red) / nf;
+        if (AHEAD) fetch(row + stride);
+        const float mu = row_sum.sum(s) / nf;
         float q = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -128,8 +174,8 @@ __global__ __launch_bounds__(BLOCK) void norm_fwd_kernel(const T* __restrict__ x
                 if (col + e < n) q = __builtin_fmaf(d, d, q);
             }
         }
-        const float r = 1.f / sqrtf(row_sum(q, tpr, red) / nf + eps);
-        if (!live) continue;
+        const float r = 1.f / sqrtf(row_sum.sum(q) / nf + eps);
+        if (row >= rows) continue;
         if (t == 0 && mean) { mean[row] = mu; rstd[row] = r; }
         T* yr = y + row * ys;
 #pragma unroll
@@ -154,7 +200,8 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(const T* __restrict__ g
                                                         int64_t rows, int n, int tpr) {
     constexpr int V = Chunk<T>::V;
     extern __shared__ float lds[];
-    __shared__ float red[2][16];
+    __shared__ float red[2][16][2];
+    RowSum row_sum = {red, tpr, 0};
     const int t = threadIdx.x & (tpr - 1), per = blockDim.x / tpr;
     const float nf = (float)n;
     float wv[C][V], aw[C][V], ab[C][V];
@@ -167,26 +214,39 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(const T* __restrict__ g
             aw[c][e] = ab[c][e] = 0.f;
         }
     }
-    for (int64_t base = (int64_t)blockIdx.x * per; base < rows; base += (int64_t)gridDim.x * per) {
-        const int64_t row = base + threadIdx.x / tpr;
-        const bool live = row < rows;
-        const int64_t at = live ? row : 0;
-        const float mu = mean[at], r = rstd[at];
-        float xh[C][V], gv[C][V], s1 = 0.f, s2 = 0.f;
+    // the next row is requested while this one is summed (131072 x 2048 bf16: 430 -> 338 us); workgroups of 1024 threads have
+    // no registers for it
+    constexpr bool AHEAD = BLOCK < 1024;
+    u32x4 ahead_x[C], ahead_g[C];
+    float mu = 0.f, r = 0.f;
+    auto fetch = [&](int64_t row) {
+        if (row < rows) { mu = mean[row]; r = rstd[row]; }
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int col = (c * tpr + t) * V;
-            if (live && col < n) {
-                load_chunk(x + at * xs + col, n - col, xh[c]);
-                load_chunk(g + at * gs + col, n - col, gv[c]);
-#pragma unroll
-                for (int e = 0; e < V; ++e) xh[c][e] = (xh[c][e] - mu) * r;
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) xh[c][e] = gv[c][e] = 0.f;
+            ahead_x[c] = ahead_g[c] = u32x4{0, 0, 0, 0};
+            if (row < rows && col < n) {
+                ahead_x[c] = load_raw(x + row * xs + col, n - col);
+                ahead_g[c] = load_raw(g + row * gs + col, n - col);
             }
+        }
+    };
+    const int64_t stride = (int64_t)gridDim.x * per;
+    int64_t row = (int64_t)blockIdx.x * per + threadIdx.x / tpr;
+    if (AHEAD) fetch(row);
+    for (int64_t base = (int64_t)blockIdx.x * per; base < rows; base += stride, row += stride) {
+        const bool live = row < rows;
+        float xh[C][V], gv[C][V], s1 = 0.f, s2 = 0.f;
+        if (!AHEAD) fetch(row);
+        const float rr = r;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int col = (c * tpr + t) * V;
+            widen<T>(ahead_x[c], xh[c]);
+            widen<T>(ahead_g[c], gv[c]);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
+                xh[c][e] = live && col < n ? (xh[c][e] - mu) * r : 0.f;
                 const float u = gv[c][e] * wv[c][e];     // (past the row's end g is 0: nothing is added)
                 s1 += u;
                 s2 = __builtin_fmaf(u, xh[c][e], s2);
@@ -194,8 +254,10 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(const T* __restrict__ g
                 ab[c][e] += gv[c][e];
             }
         }
+        if (AHEAD) fetch(row + stride);
         if (!gx) continue;
-        const float m1 = row_sum(s1, tpr, red[0]) / nf, m2 = row_sum(s2, tpr, red[1]) / nf;
+        row_sum.sum(s1, s2);
+        const float m1 = s1 / nf, m2 = s2 / nf;
         if (!live) continue;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -205,7 +267,7 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(const T* __restrict__ g
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const float u = gv[c][e] * wv[c][e];
-                    d[e] = r * ((u - m1) - xh[c][e] * m2);
+                    d[e] = rr * ((u - m1) - xh[c][e] * m2);
                 }
                 store_chunk(gx + row * gxs + col, n - col, d);
             }
@@ -242,19 +304,20 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(const T* __restrict__ g
     }
 }
 
-// grad_w = sum over the partials of their first n floats, grad_b of their second n: 16 columns x 16 slices a workgroup
-__global__ __launch_bounds__(256) void norm_reduce_kernel(const float* __restrict__ partial, int count, int n,
-                                                          float* __restrict__ gw, float* __restrict__ gb) {
-    __shared__ float sum[16][17];
-    const int64_t col = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
-    const int slice = threadIdx.x >> 4;
+// grad_w = sum over the partials of their first n floats, grad_b of their second n: 32 columns x 32 slices a workgroup
+__global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* __restrict__ partial, int count, int n,
+                                                           float* __restrict__ gw, float* __restrict__ gb) {
+    __shared__ float sum[32][33];
+    const int64_t col = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31), all = 2 * (int64_t)n;
+    const int slice = threadIdx.x >> 5;
     float s = 0.f;
-    if (col < 2 * (int64_t)n)
-        for (int k = slice; k < count; k += 16) s += partial[(int64_t)k * 2 * n + col];
-    sum[slice][threadIdx.x & 15] = s;
+    if (col < all)
+#pragma unroll 4
+        for (int k = slice; k < count; k += 32) s += partial[k * all + col];
+    sum[slice][threadIdx.x & 31] = s;
     __syncthreads();
-    if (slice == 0 && col < 2 * (int64_t)n) {
-        for (int k = 1; k < 16; ++k) s += sum[k][threadIdx.x & 15];
+    if (slice == 0 && col < all) {
+        for (int k = 1; k < 32; ++k) s += sum[k][threadIdx.x & 31];
         if (col < n) { if (gw) gw[col] = s; }
         else if (gb) gb[col - n] = s;
     }
@@ -267,7 +330,8 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(const T* __restrict
                                                              T* __restrict__ y, int64_t ys, float* __restrict__ mean,
                                                              float* __restrict__ rstd, int64_t rows, int n, float eps) {
     constexpr int V = Chunk<T>::V;
-    __shared__ float red[16];
+    __shared__ float red[2][16][2];
+    RowSum row_sum = {red, 1024, 0};
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T* xr = x + row * xs;
         float v[V], s = 0.f, q = 0.f;
@@ -276,14 +340,14 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(const T* __restrict
 #pragma unroll
             for (int e = 0; e < V; ++e) s += v[e];
         }
-        const float mu = row_sum(s, 1024, red) / (float)n;
+        const float mu = row_sum.sum(s) / (float)n;
         for (int64_t col = threadIdx.x * V; col < n; col += 1024 * V) {
             load_chunk(xr + col, (int)(n - col), v);
 #pragma unroll
             for (int e = 0; e < V; ++e)
                 if (col + e < n) q = __builtin_fmaf(v[e] - mu, v[e] - mu, q);
         }
-        const float r = 1.f / sqrtf(row_sum(q, 1024, red) / (float)n + eps);
+        const float r = 1.f / sqrtf(row_sum.sum(q) / (float)n + eps);
         if (threadIdx.x == 0 && mean) { mean[row] = mu; rstd[row] = r; }
         for (int64_t col = threadIdx.x * V; col < n; col += 1024 * V) {
             load_chunk(xr + col, (int)(n - col), v);
@@ -301,7 +365,8 @@ __global__ __launch_bounds__(1024) void norm_bwd_long_kernel(const T* __restrict
                                                              const float* __restrict__ rstd, const float* __restrict__ w,
                                                              T* __restrict__ gx, int64_t gxs, int64_t rows, int n) {
     constexpr int V = Chunk<T>::V;
-    __shared__ float red[2][16];
+    __shared__ float red[2][16][2];
+    RowSum row_sum = {red, 1024, 0};
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const float mu = mean[row], r = rstd[row];
         float xv[V], gv[V], s1 = 0.f, s2 = 0.f;
@@ -315,7 +380,8 @@ __global__ __launch_bounds__(1024) void norm_bwd_long_kernel(const T* __restrict
                 if (col + e < n) s2 = __builtin_fmaf(u, (xv[e] - mu) * r, s2);
             }
         }
-        const float m1 = row_sum(s1, 1024, red[0]) / (float)n, m2 = row_sum(s2, 1024, red[1]) / (float)n;
+        row_sum.sum(s1, s2);
+        const float m1 = s1 / (float)n, m2 = s2 / (float)n;
         for (int64_t col = threadIdx.x * V; col < n; col += 1024 * V) {
             load_chunk(x + row * xs + col, (int)(n - col), xv);
             load_chunk(g + row * gs + col, (int)(n - col), gv);
@@ -363,9 +429,11 @@ struct Split { int tpr, chunks, block, per; };
 inline Split split_of(int n, int v) {
     const int64_t need = ((int64_t)n + v - 1) / v;          // chunks of the row
     Split s = {1, 1, 256, 0};
+    const int few = v == 4 ? 4 : 1;                         // 16 floats or 8 halfs a thread, more only where 256 threads are too few
     while (s.tpr < 64 && s.tpr < need) s.tpr *= 2;
-    while (s.chunks < EMAX / v && (int64_t)s.tpr * s.chunks < need) s.chunks *= 2;
+    while (s.chunks < few && (int64_t)s.tpr * s.chunks < need) s.chunks *= 2;
     while (s.tpr < 256 && (int64_t)s.tpr * s.chunks < need) s.tpr *= 2;
+    while (s.chunks < EMAX / v && (int64_t)s.tpr * s.chunks < need) s.chunks *= 2;
     if ((int64_t)s.tpr * s.chunks < need) {
         s.tpr = s.block = 1024;
         s.chunks = (int64_t)s.tpr * (EMAX_WIDE / v) < need ? 0 : EMAX_WIDE / v;
@@ -390,8 +458,12 @@ int launch_fwd(const void* x, int64_t xs, const float* w, const float* b, void* 
                            stream, xp, xs, w, b, yp, ys, mean, rstd, rows, n, eps);
         return nf_launch_status();
     }
+    // a grid that stays: the vectors are read once a workgroup.  Eight workgroups a CU where a thread has one chunk (in long
+    // runs twice that: 131072 x 2048 bf16 276 -> 236 us, but 4099 x 1031 fp16 16 -> 20), four where it has more (131072 x 512
+    // fp32: 102 us, with eight 111), two of 1024 threads
     const int64_t need = (rows + s.per - 1) / s.per;
-    const dim3 grid((int)(need < FWD_GRID ? need : FWD_GRID)), block(s.block);
+    const int64_t most = s.block == 1024 ? 512 : s.chunks > 1 ? 1024 : need >= 16384 ? 4096 : 2048;
+    const dim3 grid((int)(need < most ? need : most)), block(s.block);
 #define NF_FWD(C, BLOCK) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_fwd_kernel<T, C, BLOCK>), grid, block, 0, stream, xp, xs, w, \
                                             b, yp, ys, mean, rstd, rows, n, eps, s.tpr)
     if (s.block == 1024) NF_FWD(EMAX_WIDE / Chunk<T>::V, 1024);
@@ -439,7 +511,7 @@ int launch_bwd(const void* g, int64_t gs, const void* x, int64_t xs, const float
     }
     int e = nf_launch_status();
     if (e || !sums) return e;
-    hipLaunchKernelGGL(norm_reduce_kernel, dim3(nf_ceil_div(2 * (int64_t)n, 16)), dim3(256), 0, stream, partial, count, n,
+    hipLaunchKernelGGL(norm_reduce_kernel, dim3(nf_ceil_div(2 * (int64_t)n, 32)), dim3(1024), 0, stream, partial, count, n,
                        gw, gb);
     return nf_launch_status();
 }

@@ -429,9 +429,10 @@ __global__ __launch_bounds__(256) void orth_sym_kernel(Plan plan, SymOps ops, fl
     const Group& g = plan.g[k];
     const int n = (g.sm + T - 1) / T, per = n * (n + 1) / 2, parts = plan.parts[k];
     const int order = xcd_order(blockIdx.x - plan.first_tile[k], plan.first_tile[k + 1] - plan.first_tile[k]);
-    const int in_group = order / parts, part = order - in_group * parts, idx = in_group / per;
+    // (a part's tiles are neighbours: they read the same rows)
+    const int idx = order / (per * parts), in_matrix = order - idx * (per * parts), part = in_matrix / per, tile = in_matrix - part * per;
     int ti, tj;
-    triangle(in_group - idx * per, n, ti, tj);
+    triangle(tile, n, ti, tj);
     const int64_t slot = (int64_t)g.count * g.sm * g.sm * CELL;
     char* slots = ws + g.s + (int64_t)idx * g.sm * g.sm * CELL;
     const bool from_x = op.p == FROM_X;
@@ -462,7 +463,7 @@ __global__ __launch_bounds__(256) void orth_sym_kernel(Plan plan, SymOps ops, fl
             if (ci >= g.sm || cj >= g.sm) continue;
             if (parts > 1) {
                 float* to = partial + plan.partial[k] +
-                            (((int64_t)blockIdx.y * per * g.count * parts + order) * (T * T) + li * T + lj) * 1024 + lane * 4;
+                            ((((int64_t)blockIdx.y * g.count + idx) * per + tile) * parts + part) * (T * T * 1024) + (li * T + lj) * 1024 + lane * 4;
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     *reinterpret_cast<float4*>(to + r * 256) = make_float4(ring.acc[i][j][4 * r], ring.acc[i][j][4 * r + 1],
