@@ -418,10 +418,11 @@ __device__ __forceinline__ void triangle(int t, int n, int& ti, int& tj) {
     tj = ti + t;
 }
 
-// Symmetric products: blockIdx.y picks the operation.  Where a group's k cells are cut into parts, a workgroup takes one
-// and leaves its raw accumulators in `partial`, which orth_sym_finish_kernel adds in order.
+// Symmetric products: blockIdx.y picks the operation.  Where a group's k cells are cut into parts (or `raw`), a workgroup takes
+// one and leaves its raw accumulators in `partial`, which orth_sym_finish_kernel or orth_chain_kernel adds in order.
 template <int T, int RING>
-__global__ __launch_bounds__(256) void orth_sym_kernel(Plan plan, SymOps ops, float* __restrict__ partial, char* __restrict__ ws) {
+__global__ __launch_bounds__(256) void orth_sym_kernel(Plan plan, SymOps ops, int raw, float* __restrict__ partial,
+                                                       char* __restrict__ ws) {
     extern __shared__ __align__(16) char lds[];
     const SymOp& op = ops.op[blockIdx.y];
     int k = 0;
@@ -461,7 +462,7 @@ __global__ __launch_bounds__(256) void orth_sym_kernel(Plan plan, SymOps ops, fl
         for (int j = 0; j < F; ++j) {
             const int li = wi * F + i, lj = wj * F + j, ci = ti * T + li, cj = tj * T + lj;
             if (ci >= g.sm || cj >= g.sm) continue;
-            if (parts > 1) {
+            if (parts > 1 || raw) {
                 float* to = partial + plan.partial[k] +
                             ((((int64_t)blockIdx.y * g.count + idx) * per + tile) * parts + part) * (T * T * 1024) + (li * T + lj) * 1024 + lane * 4;
 #pragma unroll
@@ -832,6 +833,110 @@ __device__ __forceinline__ void store_both(char* cell, char* transposed, const f
     }
 }
 
+// The m x m side of a block of steps in one launch, for sides up to 128: a workgroup of eight waves per matrix, the operands of
+// a product in two places of the LDS, every matrix's own values in fp32 registers (a wave has up to two cells i <= j of each).
+// S comes as raw accumulators; T of alpha I + T goes to slot 0, scaled for MixOp.  Nine products of 128 x 128 take 27 us, bound by
+// the LDS, against nine launches of 5 us and more.
+template <int SM>
+__global__ __launch_bounds__(512) void orth_chain_kernel(Plan plan, int block, const float* __restrict__ partial, char* __restrict__ ws) {
+    constexpr int SYM = (SM * (SM + 1) / 2 + 7) / 8;
+    extern __shared__ __align__(16) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int k = 0;
+    while (k + 1 < plan.groups && (int)blockIdx.x >= plan.first_tile[k + 1]) ++k;
+    const Group& g = plan.g[k];
+    const int idx = blockIdx.x - plan.first_tile[k], parts = plan.parts[k], sm = g.sm;
+    char *p = lds, *q = lds + SM * SM * CELL;
+    int ci[SYM], cj[SYM];
+#pragma unroll
+    for (int u = 0; u < SYM; ++u) {
+        int t = u * 8 + wave, i = 0;
+        while (i < sm && t >= sm - i) t -= sm - i++;
+        ci[u] = i;                                       // (sm: none)
+        cj[u] = i + t;
+    }
+    struct Sym { f32x16 v[SYM]; };
+    auto put = [&](char* to, const Sym& m, float scale) {
+#pragma unroll
+        for (int u = 0; u < SYM; ++u)
+            if (ci[u] < sm) store_both(to + (ci[u] * SM + cj[u]) * CELL, to + (cj[u] * SM + ci[u]) * CELL, m.v[u], scale, lane);
+    };
+    // a A + b B + scale * (the product of what two places hold)
+    auto mix = [&](const char* x, const char* y, float scale, float a, const Sym& ma, float b, const Sym& mb) {
+        Sym r;
+#pragma unroll
+        for (int u = 0; u < SYM; ++u)
+            if (ci[u] < sm) r.v[u] = a * ma.v[u] + (b * mb.v[u] + scale * cell_product(x + ci[u] * SM * CELL, y + cj[u] * SM * CELL, sm, lane));
+        return r;
+    };
+    Sym s;
+#pragma unroll
+    for (int u = 0; u < SYM; ++u) {
+        if (ci[u] >= sm) continue;
+        const float* from = partial + plan.partial[k] + (int64_t)idx * parts * (16 * 1024) + (ci[u] * 4 + cj[u]) * 1024 + lane * 4;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s.v[u][r] = 0.f;
+#pragma unroll 4
+        for (int part = 0; part < parts; ++part, from += 16 * 1024)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float4 v = *reinterpret_cast<const float4*>(from + r * 256);
+                s.v[u][4 * r] += v.x;
+                s.v[u][4 * r + 1] += v.y;
+                s.v[u][4 * r + 2] += v.z;
+                s.v[u][4 * r + 3] += v.w;
+            }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s.v[u][r] *= 0x1p-30f;
+    }
+    put(p, s, 0x1p15f);
+    __syncthreads();
+    Sym t = mix(p, p, CC * 0x1p-30f, CB, s, 0.f, s);     // B = b S + c S S
+    float scale = 0x1p14f;
+    if (block > 1) {
+        put(q, t, 0x1p14f);                              // q: B
+        __syncthreads();
+        Sym m = mix(q, p, 0x1p-29f, CA, s, 0.f, s);      // M = a S + B S
+        __syncthreads();
+        put(p, m, 0x1p15f);
+        __syncthreads();
+        s = mix(q, p, 0x1p-29f, CA, m, 0.f, m);          // S' = a M + B M
+        __syncthreads();
+        put(p, s, 0x1p15f);
+        __syncthreads();
+        Sym b = mix(p, p, CC * 0x1p-30f, CB, s, 0.f, s); // B'
+        __syncthreads();
+        put(p, b, 0x1p14f);
+        __syncthreads();
+        t = mix(p, q, 0x1p-28f, CA, t, CA, b);           // T' = a B + a B' + B' B
+        scale = 0x1p11f;
+        if (block > 2) {
+            __syncthreads();
+            put(q, s, 0x1p15f);
+            __syncthreads();
+            m = mix(p, q, 0x1p-29f, CA, s, 0.f, s);      // M'
+            __syncthreads();
+            put(q, m, 0x1p15f);
+            __syncthreads();
+            s = mix(p, q, 0x1p-29f, CA, m, 0.f, m);      // S''
+            __syncthreads();
+            put(q, s, 0x1p15f);
+            __syncthreads();
+            b = mix(q, q, CC * 0x1p-30f, CB, s, 0.f, s); // B''
+            __syncthreads();
+            put(q, b, 0x1p14f);
+            put(p, t, 0x1p11f);
+            __syncthreads();
+            t = mix(q, p, 0x1p-25f, CA, t, CA * CA, b);  // T'' = a T' + a^2 B'' + B'' T'
+            scale = 0x1p9f;
+        }
+    }
+    char* out = ws + g.s + (int64_t)idx * sm * sm * CELL;
+#pragma unroll
+    for (int u = 0; u < SYM; ++u)
+        if (ci[u] < sm) store_both(out + (ci[u] * sm + cj[u]) * CELL, out + (cj[u] * sm + ci[u]) * CELL, t.v[u], scale, lane);
+}
+
 template <int SM, int NC, typename T, bool MUON>
 __global__ __launch_bounds__(512) void orth_small_kernel(Group g, Pointers ptr, Ends io, int steps, double eps) {
     constexpr int SYM = (SM * (SM + 1) / 2 + 7) / 8;     // cells i <= j of S a wave
@@ -1006,7 +1111,7 @@ int cut_mix(Plan& plan, int64_t& tiles) {
 
 // T of a launch of symmetric products; sets the plan's workgroups and parts, and the floats that the parts' accumulators
 // take
-int cut_sym(Plan& plan, bool from_x, int64_t& workgroups, int64_t& floats) {
+int cut_sym(Plan& plan, bool from_x, bool raw, int64_t& workgroups, int64_t& floats) {
     floats = 0;
     int64_t work = 0, most = 0;
     for (int k = 0; k < plan.groups; ++k) plan.parts[k] = 1;
@@ -1022,7 +1127,7 @@ int cut_sym(Plan& plan, bool from_x, int64_t& workgroups, int64_t& floats) {
     int64_t share = (work + 2 * CUS - 1) / (2 * CUS);
     if (share < 16) share = 16;
     workgroups = tiles;
-    if (most >= share + share / 2) {
+    if (raw || most >= share + share / 2) {
         workgroups = 0;
         for (int k = 0; k < plan.groups; ++k) {
             const Group& g = plan.g[k];
@@ -1032,12 +1137,13 @@ int cut_sym(Plan& plan, bool from_x, int64_t& workgroups, int64_t& floats) {
             plan.first_tile[k] = workgroups > 0x7fffffff ? 0x7fffffff : (int)workgroups;
             plan.partial[k] = floats;
             workgroups += count * parts;
-            if (parts > 1) floats += 2 * count * parts * 16 * 1024;              // (two operations in a launch)
+            if (raw) floats += count * parts * 16 * 1024;
+            else if (parts > 1) floats += 2 * count * parts * 16 * 1024;         // (two operations in a launch)
         }
         plan.first_tile[plan.groups] = workgroups > 0x7fffffff ? 0x7fffffff : (int)workgroups;
         return 4;
     }
-    // short k loops (up to 512) leave a large tile's start and end uncovered: four small ones on its CU overlap them
+    // short k loops (up to 512) leave a large tile's start and end uncovered: small ones on the same CU overlap them
     if (tiles >= CUS / 2 && most > 16) return 4;
     workgroups = count_tiles(plan, 2, 2, true);
     return 2;
@@ -1064,7 +1170,15 @@ int next_block(const Plan& plan, bool exact, int done, int steps) {
     return left < most ? left : most;
 }
 
-constexpr int SLOTS_ONE = 2, SLOTS_TWO = 4, SLOTS_THREE = 5;
+constexpr int SLOTS_CHAIN = 1, SLOTS_ONE = 2, SLOTS_TWO = 4, SLOTS_THREE = 5;
+
+// Whether the m x m side is orth_chain_kernel's: all its matrices within 4 x 4 cells, and blocks of steps to save launches in
+// (step by step it has one product, which two launches of 5 us do as fast).
+bool chained(const Plan& plan, bool exact) {
+    for (int k = 0; k < plan.groups; ++k)
+        if (plan.g[k].sm > 4) return false;
+    return next_block(plan, exact, 0, 3) > 1;
+}
 
 // the tiny groups' workgroups and parts; the doubles of their partial sums (0: one launch does it all)
 int64_t cut_tiny(Plan& plan) {
@@ -1100,11 +1214,12 @@ size_t layout(Plan& plan, Plan& tiny, bool exact, int64_t& partial) {
     int64_t most = 0;
     for (int from_x = 0; from_x < 2; ++from_x) {
         int64_t workgroups, floats;
-        cut_sym(plan, from_x, workgroups, floats);
+        if (chained(plan, exact) && !from_x) continue;
+        cut_sym(plan, from_x, chained(plan, exact), workgroups, floats);
         most = floats > most ? floats : most;
     }
     at += most * sizeof(float);
-    const int block = next_block(plan, exact, 0, 3), slots = block == 3 ? SLOTS_THREE : block == 2 ? SLOTS_TWO : SLOTS_ONE;
+    const int block = next_block(plan, exact, 0, 3), slots = chained(plan, exact) ? SLOTS_CHAIN : block == 3 ? SLOTS_THREE : block == 2 ? SLOTS_TWO : SLOTS_ONE;
     for (int k = 0; k < plan.groups; ++k) {
         Group& g = plan.g[k];
         const int64_t x = (int64_t)g.count * g.sm * g.sn * CELL, s = (int64_t)g.count * g.sm * g.sm * CELL;
@@ -1129,7 +1244,7 @@ struct Job {
 };
 
 template <int T, int RING>
-int launch_sym(const Job& job, const SymOps& ops, int count, int64_t workgroups, bool parts) {
+int launch_sym(const Job& job, const SymOps& ops, int count, int64_t workgroups, bool parts, bool raw) {
     constexpr size_t lds = (size_t)RING * T * 4 * PIECE;
     static unsigned long long done;
     if (lds > 64 * 1024) {
@@ -1138,9 +1253,9 @@ int launch_sym(const Job& job, const SymOps& ops, int count, int64_t workgroups,
     }
     float* partial = (float*)(job.ws + job.partial);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_sym_kernel<T, RING>), dim3((unsigned)workgroups, count), dim3(256), lds, job.stream,
-                       job.plan, ops, partial, job.ws);
+                       job.plan, ops, (int)raw, partial, job.ws);
     const int e = nf_launch_status();
-    if (e || !parts) return e;
+    if (e || !parts || raw) return e;
     if constexpr (T == 4) {
         Plan plan = job.plan;                            // the groups with parts, a wave a cell
         int64_t total = 0;
@@ -1164,12 +1279,41 @@ int launch_sym(const Job& job, const SymOps& ops, int count, int64_t workgroups,
     return NF_OK;
 }
 
-int sym(Job& job, const SymOps& ops, int count) {
+int sym(Job& job, const SymOps& ops, int count, bool raw = false) {
     int64_t workgroups, floats;
-    const int t = cut_sym(job.plan, ops.op[0].p == FROM_X, workgroups, floats);
+    const int t = cut_sym(job.plan, ops.op[0].p == FROM_X, raw, workgroups, floats);
     if (workgroups > 0x7fffffff) return NF_ERR_SHAPE;
-    if (t == 4) return launch_sym<4, 4>(job, ops, count, workgroups, floats != 0);
-    return launch_sym<2, 4>(job, ops, count, workgroups, false);
+    if (t == 4) return launch_sym<4, 4>(job, ops, count, workgroups, floats != 0, raw);
+    return launch_sym<2, 4>(job, ops, count, workgroups, false, false);
+}
+
+template <int SM>
+int launch_chain(const Job& job, const Plan& plan, int block) {
+    constexpr int lds = 2 * SM * SM * CELL;
+    if (lds > 64 * 1024) {
+        static unsigned long long done;
+        const int e = nf_raise_lds_cap((const void*)orth_chain_kernel<SM>, &done);
+        if (e) return e;
+    }
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_chain_kernel<SM>), dim3((unsigned)plan.first_tile[plan.groups]), dim3(512), lds, job.stream,
+                       plan, block, (const float*)(job.ws + job.partial), job.ws);
+    return nf_launch_status();
+}
+
+int chain(Job& job, int block) {
+    const SymOp op = {FROM_X, FROM_X, 0, NONE, NONE, 1.f, 0.f, 0.f};
+    int e = sym(job, SymOps{{op, op}}, 1, true);
+    if (e) return e;
+    Plan plan = job.plan;                                // a workgroup a matrix
+    int64_t total = 0;
+    int most = 0;
+    for (int k = 0; k < plan.groups; ++k) {
+        plan.first_tile[k] = (int)total;
+        total += plan.g[k].count;
+        most = plan.g[k].sm > most ? plan.g[k].sm : most;
+    }
+    plan.first_tile[plan.groups] = (int)total;
+    return most <= 2 ? launch_chain<2>(job, plan, block) : launch_chain<4>(job, plan, block);
 }
 
 int sym(Job& job, SymOp op) { return sym(job, SymOps{{op, op}}, 1); }
@@ -1290,6 +1434,14 @@ int run(Job& job) {
     for (int s = 0, to = 1; s < job.steps; to ^= 1) {
         const int block = next_block(plan, OUT == OUT_F32, s, job.steps);
         MixOp op;
+        if (chained(plan, OUT == OUT_F32)) {
+            if ((e = chain(job, block))) return e;
+            op = block == 1 ? MixOp{0, to, CA * TWO(14), TWO(-14)}
+                            : block == 2 ? MixOp{0, to, a2 * TWO(11), TWO(-11)} : MixOp{0, to, a2 * CA * TWO(9), TWO(-9)};
+            s += block;
+            if ((e = s < job.steps ? mix<OUT_X>(job, op) : mix<OUT>(job, op))) return e;
+            continue;
+        }
         if ((e = sym(job, {FROM_X, FROM_X, 0, NONE, NONE, TWO(-15), 0.f, 0.f}))) return e;            // S = X X^T
         if ((e = sym(job, {0, 0, 1, 0, NONE, CC * TWO(-16), CB / CC * TWO(15), 0.f}))) return e;            // B
         if (block == 1) {

@@ -141,7 +141,7 @@ def test_overlap_check():
 @pytest.mark.gpu
 @pytest.mark.parametrize('kind', TYPES, ids=lambda t: str(t)[6:])
 @pytest.mark.parametrize('shape', [(1, 1), (1, 7), (7, 1), (2, 3), (31, 33), (32, 32), (2, 33, 129), (129, 33), (64, 64),
-                                   (3, 65, 640), (1000, 300), (2, 517, 1031), (5, 40, 50, 30), (700, 17, 5), (40, 8000), (3, 32, 700), (900, 31), (5, 40000), (2, 2000, 12), (3, 96, 100), (128, 128), (288, 64), (96, 190), (33, 97), (60, 200), (120, 129),
+                                   (3, 65, 640), (1000, 300), (2, 517, 1031), (5, 40, 50, 30), (700, 17, 5), (40, 8000), (3, 32, 700), (900, 31), (5, 40000), (2, 2000, 12), (3, 96, 100), (128, 128), (288, 64), (96, 190), (33, 97), (60, 200), (120, 129), (2, 50, 3000), (1500, 100), (128, 700),
                                    (20, 512, 512)], ids=str)
 def test_orthogonalize(shape, kind):
     g = gradients(shape, sum(shape)).to(kind)
