@@ -4,7 +4,8 @@
     python -m torch.distributed.run --nproc-per-node N --master-addr 127.0.0.1 benchmarks/bench_train.py
 
 One step = forward (-mean log_prob) + backward through the hand-written kernels + bucketed gradient
-all-reduce over RCCL (when WORLD_SIZE > 1) + Adam.  Per-GPU batch is fixed (weak scaling)."""
+all-reduce over RCCL (when WORLD_SIZE > 1) + Adam, or with --optimizer muon Muon for the weight matrices and Adam for the
+biases.  Per-GPU batch is fixed (weak scaling)."""
 import argparse
 import json
 import os
@@ -30,6 +31,8 @@ def main():
                     help='final layer + spline of the training forward as two autograd nodes (A/B of the fused forward)')
     ap.add_argument('--fused-forward-f16x2', action='store_true',
                     help='f16x2 mode: the one-launch training forward on the t4 kernel (off by default: slower end to end)')
+    ap.add_argument('--optimizer', default='adam', choices=['adam', 'muon'],
+                    help='muon: nf.Muon for the weight matrices, Adam for the biases')
     args = ap.parse_args()
     from normalizing_flows_amd import transforms as _tr
     if args.two_launch_forward:
@@ -51,7 +54,9 @@ def main():
               for _ in range(args.layers)]
     flow = nf.BaseNeuralSplineFlow(nf.CompositeTransform(layers), nf.StandardNormal([D])).cuda()
     # (torch's single-launch Adam: the default multi-tensor path is 12 launches of 35-65 us per step here)
-    opt = torch.optim.Adam(flow.parameters(), lr=1e-4, fused=True)
+    matrices = [p for p in flow.parameters() if p.dim() == 2] if args.optimizer == 'muon' else []
+    rest = [p for p in flow.parameters() if p.dim() != 2 or not matrices]
+    opts = [torch.optim.Adam(rest, lr=1e-4, fused=True)] + ([nf.Muon(matrices, lr=1e-3)] if matrices else [])
     x = torch.randn(args.batch, D, device='cuda', generator=torch.Generator(device='cuda').manual_seed(99 + rank))
     losses = []
     # gradients live in flat buckets; with several ranks their all-reduces start from per-parameter hooks while backward
@@ -63,7 +68,8 @@ def main():
         loss = -flow.log_prob(x).mean()
         loss.backward()
         sync.finish()
-        opt.step()
+        for opt in opts:
+            opt.step()
         return loss
 
     for _ in range(args.warmup):
@@ -80,7 +86,8 @@ def main():
         dist.barrier()
     dt = time.perf_counter() - t0
     if rank == 0:
-        print(json.dumps({'metric': 'training samples/sec (fwd+bwd+allreduce+Adam), RQ-spline MAF D=784',
+        print(json.dumps({'metric': 'training samples/sec (fwd+bwd+allreduce+%s), RQ-spline MAF D=784' %
+                          args.optimizer.capitalize(),
                           'value': world * args.batch * args.steps / dt, 'unit': 'samples/s', 'n_gpus': world,
                           'ms_per_step': 1e3 * dt / args.steps, 'batch_per_gpu': args.batch, 'dtype': args.dtype,
                           'losses': losses, 'peak_mem_gb': torch.cuda.max_memory_allocated() / 2**30}))

@@ -2,6 +2,7 @@
 // in Python costs 60 us and more a training step before any kernel runs (this one: 20 us).  The work itself is in libnf_hip.so
 // (include/nf_hip.h), whose entry points the package hands over once it has loaded that library.
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
@@ -113,6 +114,18 @@ std::optional<Tensor> vector(const std::optional<Tensor>& t, const char* name, c
     return t->contiguous();
 }
 
+// A leaf whose gradient an earlier graph, still alive, accumulates on another stream: a backward pass captured with it would
+// wait for that stream from inside the capture, which ends the process.  Refused here, before anything is recorded.
+void check_capture(const Tensor& t, const char* name) {
+    if (!t.is_leaf() || !t.requires_grad()) return;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!accumulator) return;
+    const auto stream = accumulator->stream();
+    TORCH_CHECK(!stream || stream->id() == c10::hip::getCurrentHIPStream(t.get_device()).id(), name,
+                " takes part in an autograd graph that was recorded on another stream and is still alive: delete that graph's "
+                "outputs before capturing a training step");
+}
+
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
     TORCH_CHECK(lib.fwd, "libnf_hip.so is not loaded");
     TORCH_CHECK(x.is_cuda(), "x must be a tensor on the GPU (MI355X); this package has no CPU path");
@@ -126,6 +139,14 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
     const Tensor rows = unit_rows(x.dim() == 2 ? x : x.reshape({-1, x.size(-1)}));
     const bool records = at::GradMode::is_enabled() && (x.requires_grad() || (w && w->requires_grad()) ||
                                                         (b && b->requires_grad()));
+    if (records) {
+        const c10::DeviceGuard guard(x.device());
+        if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+            check_capture(x, "x");
+            if (w) check_capture(*weight, "weight");
+            if (b) check_capture(*bias, "bias");
+        }
+    }
     const Tensor y = records ? LayerNormNode::apply(rows, w, b, eps)
                              : normalise(rows, w.value_or(Tensor()), b.value_or(Tensor()), eps, nullptr);
     return x.dim() == 2 ? y : y.view(x.sizes());

@@ -267,6 +267,29 @@ def test_captured_step():
         assert all(torch.equal(p, q) for p, q in zip(got, call()))
 
 
+@pytest.mark.gpu
+def test_capture_with_a_live_eager_graph_is_refused():
+    """A leaf that an eager graph on another stream still holds: the forward call inside the capture says so (its backward
+    pass would end the process); without that graph the same capture works."""
+    m = nf.LayerNorm(40).cuda()
+    x = torch.randn(30, 40, device='cuda')
+    alive = m(x).sum()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match='still alive'):
+            m(x)
+        kept = x + 1
+    graph.replay()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = m(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        assert torch.equal(y, m(x)) and torch.equal(kept, x + 1)
+
+
 def _plain_net(net, x, context=None):
     """ResidualNet(use_layer_norm=True) from its state in float64 torch operations."""
     p = {k: v.detach().cpu().double().requires_grad_() for k, v in net.named_parameters()}
@@ -288,8 +311,9 @@ def _plain_net(net, x, context=None):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('mode', ['f32', 'f16x2'])
 @pytest.mark.parametrize('context', [None, 3])
-def test_residual_net_with_layer_norm(context):
+def test_residual_net_with_layer_norm(context, mode):
     """Values and every parameter's gradient of the conditioner against the same network in float64.  ReLU's corners: the
     inputs are drawn so that no pre-activation lies within 1e-4 of 0, which the fp32 run cannot move across."""
     torch.manual_seed(4)
@@ -302,14 +326,19 @@ def test_residual_net_with_layer_norm(context):
     want, p = _plain_net(net, x.double(), None if c is None else c.double())
     g = torch.randn(64, 10)
     grads = torch.autograd.grad(want, list(p.values()), g.double())
-    out = net(x.cuda(), None if c is None else c.cuda())
-    got = torch.autograd.grad(out, list(net.parameters()), g.cuda())
+    nf.set_matmul_dtype(mode)
+    try:
+        out = net(x.cuda(), None if c is None else c.cuda())
+        got = torch.autograd.grad(out, list(net.parameters()), g.cuda())
+        with torch.no_grad():
+            again = net(x.cuda(), None if c is None else c.cuda())
+    finally:
+        nf.set_matmul_dtype('f32')
     # (fp32 through ten layers: 2^-24 times the about 100 roundings on a path, relative to the largest value)
     assert ((out.detach().cpu().double() - want).abs().max() / want.abs().max()).item() < 100 * U * 10
     for name, a, b in zip(p, got, grads):
         assert (a.cpu().double() - b).abs().max() <= 2e-3 * b.abs().max() + 1e-6, name
-    with torch.no_grad():
-        assert torch.equal(net(x.cuda(), None if c is None else c.cuda()), out)
+    assert torch.equal(again, out)
 
 
 @pytest.mark.gpu
