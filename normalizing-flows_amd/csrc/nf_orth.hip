@@ -44,7 +44,7 @@ struct Group {
     int sm, sn;                          // cells along each
     int trans;                           // rows > columns: X = G^T
     int count, first;                    // matrices, index of the first
-    int64_t x, xt[2], s;                 // byte offsets in the workspace: X, X^T (two), the slots of m x m matrices, each
+    int64_t x, xt0, xt1, s;               // byte offsets in the workspace: X, X^T (two), the slots of m x m matrices, each
                                          // of them `count` matrices one behind the other
 };
 struct Plan {
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256) void orth_start_kernel(Plan plan, Pointers ptr
     }
     wave_sync();
     char* x = ws + g.x + ((int64_t)idx * cells + (int64_t)ci * g.sn + cj) * CELL;
-    char* xt = ws + g.xt[0] + ((int64_t)idx * cells + (int64_t)cj * g.sm + ci) * CELL;
+    char* xt = ws + g.xt0 + ((int64_t)idx * cells + (int64_t)cj * g.sm + ci) * CELL;
     sub.store<false>(x, lane);
     sub.store<true>(xt, lane);
 }
@@ -532,7 +532,7 @@ __global__ __launch_bounds__(256, 2) void orth_mix_kernel(Plan plan, Pointers pt
     constexpr int FI = TI / 2, FJ = TJ / 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave >> 1, wj = wave & 1;
     const int64_t row_bytes = (int64_t)g.sm * CELL;
-    const char* xt = ws + g.xt[op.to ^ 1] + xm;
+    const char* xt = ws + (op.to ? g.xt0 : g.xt1) + xm;
     // X's own part from the rows of X^T that were Q's, from cache; with many cells a wave, only when the fragments are done
     typename Ring<TI, TJ, RING>::Terms e;
     auto own = [&]() { ring.load(e, xt, row_bytes, ti * TI + wi * FI, tj * TJ + wj * FJ, g.sm, g.sn); };
@@ -570,7 +570,7 @@ __global__ __launch_bounds__(256, 2) void orth_mix_kernel(Plan plan, Pointers pt
             put_acc<OUT == OUT_X>(sub, lane, ring.acc[i][j], op.out_scale * (OUT == OUT_X ? 1.f : 0x1p-15f));
             if constexpr (OUT == OUT_X) {
                 sub.store<false>(ws + g.x + xm + ((int64_t)ci * g.sn + cj) * CELL, lane);
-                sub.store<true>(ws + g.xt[op.to] + xm + ((int64_t)cj * g.sm + ci) * CELL, lane);
+                sub.store<true>(ws + (op.to ? g.xt1 : g.xt0) + xm + ((int64_t)cj * g.sm + ci) * CELL, lane);
             } else {
                 const int r0 = (g.trans ? cj : ci) * 32, c0 = (g.trans ? ci : cj) * 32;
                 if (wide) {
@@ -1224,8 +1224,8 @@ size_t layout(Plan& plan, Plan& tiny, bool exact, int64_t& partial) {
         Group& g = plan.g[k];
         const int64_t x = (int64_t)g.count * g.sm * g.sn * CELL, s = (int64_t)g.count * g.sm * g.sm * CELL;
         g.x = at;
-        g.xt[0] = at + x;
-        g.xt[1] = at + 2 * x;
+        g.xt0 = at + x;
+        g.xt1 = at + 2 * x;
         g.s = at + 3 * x;
         at = g.s + slots * s;
     }
@@ -1284,7 +1284,7 @@ int sym(Job& job, const SymOps& ops, int count, bool raw = false) {
     const int t = cut_sym(job.plan, ops.op[0].p == FROM_X, raw, workgroups, floats);
     if (workgroups > 0x7fffffff) return NF_ERR_SHAPE;
     if (t == 4) return launch_sym<4, 4>(job, ops, count, workgroups, floats != 0, raw);
-    return launch_sym<2, 4>(job, ops, count, workgroups, false, false);
+    return launch_sym<2, 6>(job, ops, count, workgroups, false, false);
 }
 
 template <int SM>
@@ -1338,7 +1338,7 @@ int mix(Job& job, const MixOp& op) {
     if (tiles > 0x7fffffff) return NF_ERR_SHAPE;
     if (t == 8) return launch_mix<8, 4, 3, OUT>(job, op, tiles);
     if (t == 4) return launch_mix<4, 4, 4, OUT>(job, op, tiles);
-    return launch_mix<2, 2, 4, OUT>(job, op, tiles);
+    return launch_mix<2, 2, 6, OUT>(job, op, tiles);
 }
 
 // Scales (powers of two) of the slots: S and M = R S 15 (|M| < 1.45), B = b S + c S S 14, and of alpha I + T, the product of

@@ -2,14 +2,14 @@
 
 Tolerances are counted, not tuned.  With h = eps / 2 of the element type (one rounding of the result) and u = 2^-24 (one
 fp32 rounding):
-  * a row sum of the kernels has at most E adds in a thread and 16 between threads, E <= 32 for rows up to 16384 elements
-    and n / 1024 + 4 above: its error is at most (E + 16) u times the sum of magnitudes.  mu is then off by
-    (E + 18) u max|x|, x - mu by that and one rounding, r (whose argument is a mean of squares) by (E + 20) u relative;
-  * y = xh w + b: |dy| <= h |y| + K u [(1 + max|x| r)(1 + |xh|) |w| + |b|], K = E + 24;
+  * a row sum of the kernels has at most E adds in a thread and 22 between threads (6 in a wave, 16 waves), E <= 32 for rows up
+    to 16384 elements and n / 1024 + 4 above: its error is at most (E + 22) u times the sum of magnitudes.  mu is then off by
+    (E + 24) u max|x|, x - mu by that and one rounding, r (whose argument is a mean of squares) by (E + 26) u relative;
+  * y = xh w + b: |dy| <= h |y| + K u [(1 + max|x| r)(1 + |xh|) |w| + |b|], K = E + 30;
   * grad_x = r (u - mean u - xh mean(u xh)): two sums more, each over products with xh:
     |dgx| <= h |gx| + 4 K u r (1 + max|x| r)(1 + max|xh|)^2 max|u|;
-  * grad_w adds at most rows / 512 + 3 terms in a thread (the grid is 512 workgroups), 256 in a workgroup and 48 in the
-    second launch: |dgw| <= (rows / 512 + 320 + K (1 + max|x| r)) u sum|g| (1 + |xh|), and grad_b likewise.
+  * grad_w adds at most rows / 1024 + 1 terms in a thread (the grid is 1024 workgroups), 256 in a workgroup and 64 in the second
+    launch: |dgw| <= (rows / 1024 + 321 + K (1 + max|x| r)) u sum|g| (1 + |xh|), and grad_b likewise.
 """
 import pytest
 import torch
@@ -38,7 +38,7 @@ def bounds(x, w, b, g, kind, eps=1e-5):
     y, gx, gw, gb, xh, r = oracle(x, w, b, g, eps)
     rows, n = x.shape
     h = torch.finfo(kind).eps / 2
-    k = (32 if n <= 16384 else n / 1024 + 4) + 24
+    k = (32 if n <= 16384 else n / 1024 + 4) + 30
     wd = torch.ones(n, dtype=torch.float64) if w is None else w.double()
     bd = torch.zeros(n, dtype=torch.float64) if b is None else b.double()
     tiny = torch.finfo(kind).tiny * torch.finfo(kind).eps           # a step below the smallest normal number
@@ -48,7 +48,7 @@ def bounds(x, w, b, g, kind, eps=1e-5):
     most = (g.double() * wd).abs().amax(-1, keepdim=True) if rows else r
     tx = h * gx.abs() + 4 * k * U * r * lift * top * most + tiny
     worst = lift.max().item() if rows else 1.0
-    chain = rows / 512 + 320 + k * worst
+    chain = rows / 1024 + 321 + k * worst
     tw = chain * U * (g.double().abs() * (1 + xh.abs())).sum(0)
     tb = chain * U * g.double().abs().sum(0)
     return (y, ty), (gx, tx), (gw, tw), (gb, tb)

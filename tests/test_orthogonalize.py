@@ -157,8 +157,9 @@ def test_large_matrix():
 
 
 @pytest.mark.gpu
-def test_steps_eps_and_scale():
-    g = gradients((70, 90), 1)
+@pytest.mark.parametrize('shape', [(70, 90), (20, 300), (150, 140), (80, 700)], ids=str)
+def test_steps_eps_and_scale(shape):
+    g = gradients(shape, 1)
     for steps in (1, 2, 7):
         check(nf.orthogonalize(g, steps=steps), g, torch.float32, steps=steps)
     check(nf.orthogonalize(g, eps=0.5), g, torch.float32, eps=0.5)
@@ -176,12 +177,13 @@ def test_singular_values_come_near_one():
 
 
 @pytest.mark.gpu
-def test_special_values_stay_in_their_matrix():
-    g = gradients((5, 40, 70), 2)
+@pytest.mark.parametrize('shape', [(5, 20, 70), (5, 700, 9), (5, 40, 70), (5, 130, 150), (5, 70, 900)], ids=str)
+def test_special_values_stay_in_their_matrix(shape):
+    g = gradients(shape, 2)
     want = nf.orthogonalize(g)
     h = g.clone()
     h[1] = 0
-    h[2, 39, 69] = float('nan')
+    h[2, -1, -1] = float('nan')
     h[3, 0, 0] = float('inf')
     out = nf.orthogonalize(h)
     assert torch.equal(out[0], want[0]) and torch.equal(out[4], want[4])
