@@ -19,7 +19,6 @@ namespace {
 
 constexpr int EMAX = 32;                 // elements of a row that a thread keeps, in workgroups up to 256 threads
 constexpr int EMAX_WIDE = 16;            // in larger ones, whose threads have at most 128 registers
-constexpr int BWD_GRID = 1024;           // workgroups of the backward pass: each leaves a partial sum of 2 N floats
 constexpr int LONG_SLICES = 64;          // row slices of the long rows' weight gradient
 
 // 16 bytes of elements at the element's own alignment (global memory takes unaligned 16-byte accesses: odd row strides
@@ -63,6 +62,18 @@ __device__ __forceinline__ void store_chunk(T* p, int left, const float* v) {
 #pragma unroll
         for (int k = 0; k < V; ++k)
             if (k < left) p[k] = (T)v[k];
+    }
+}
+
+// a chunk's part of a vector of floats (nullptr: `other` throughout)
+template <int V>
+__device__ __forceinline__ void load_vector(const float* p, int col, int n, float other, float* v) {
+    if (p && col + V <= n) {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) widen<float>(load_raw(p + col + k, 4), v + k);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = p && col + k < n ? p[col + k] : other;
     }
 }
 
@@ -129,15 +140,11 @@ __global__ __launch_bounds__(BLOCK) void norm_fwd_kernel(const T* __restrict__ x
     float wv[C][V], bv[C][V];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const int col = (c * tpr + t) * V;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            wv[c][e] = (w && col + e < n) ? w[col + e] : 1.f;
-            bv[c][e] = (b && col + e < n) ? b[col + e] : 0.f;
-        }
+        load_vector<V>(w, (c * tpr + t) * V, n, 1.f, wv[c]);
+        load_vector<V>(b, (c * tpr + t) * V, n, 0.f, bv[c]);
     }
     // the next row is requested while this one is summed where one workgroup fills a CU; smaller ones cover each other, and
-    // its registers would cost them more (131072 x 2048 bf16: 236 us without, 278 with)
+    // its registers would cost them more (131072 x 2048 bf16 at one grid: 236 us without, 278 with)
     constexpr bool AHEAD = BLOCK == 1024;
     u32x4 ahead[C];
     auto fetch = [&](int64_t row) {
@@ -207,12 +214,9 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(const T* __restrict__ g
     float wv[C][V], aw[C][V], ab[C][V];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const int col = (c * tpr + t) * V;
+        load_vector<V>(w, (c * tpr + t) * V, n, 1.f, wv[c]);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            wv[c][e] = (w && col + e < n) ? w[col + e] : 1.f;
-            aw[c][e] = ab[c][e] = 0.f;
-        }
+        for (int e = 0; e < V; ++e) aw[c][e] = ab[c][e] = 0.f;
     }
     // the next row is requested while this one is summed (131072 x 2048 bf16: 430 -> 338 us); workgroups of 1024 threads have
     // no registers for it
@@ -442,9 +446,12 @@ inline Split split_of(int n, int v) {
     return s;
 }
 
+// workgroups of the backward pass
 inline int64_t bwd_groups(int64_t rows, const Split& s) {
-    const int64_t need = (rows + s.per - 1) / s.per;
-    return need < BWD_GRID ? need : BWD_GRID;
+    // each leaves a partial sum of 2 N floats, so no more than fit: four a CU; one where its threads take the registers of two
+    // or more (16384 x 8192 bf16 forward + backward: 278 us, with 1024 of them 323)
+    const int64_t need = (rows + s.per - 1) / s.per, most = s.block == 1024 || s.chunks >= 4 ? 256 : 1024;
+    return need < most ? need : most;
 }
 
 template <typename T>
@@ -458,11 +465,10 @@ int launch_fwd(const void* x, int64_t xs, const float* w, const float* b, void* 
                            stream, xp, xs, w, b, yp, ys, mean, rstd, rows, n, eps);
         return nf_launch_status();
     }
-    // a grid that stays: the vectors are read once a workgroup.  Eight workgroups a CU where a thread has one chunk (in long
-    // runs twice that: 131072 x 2048 bf16 276 -> 236 us, but 4099 x 1031 fp16 16 -> 20), four where it has more (131072 x 512
-    // fp32: 102 us, with eight 111), two of 1024 threads
-    const int64_t need = (rows + s.per - 1) / s.per;
-    const int64_t most = s.block == 1024 ? 512 : s.chunks > 1 ? 1024 : need >= 16384 ? 4096 : 2048;
+    // The vectors are read once a workgroup.  Where a thread has one chunk that is little, and more workgroups than fit keep the
+    // memory evenly busy (131072 x 2048 bf16: 207 us with 8192 of them, 276 with 2048); with more chunks four a CU
+    // (131072 x 512 fp32: 98 us, with eight 107), of 1024 threads two.
+    const int64_t need = (rows + s.per - 1) / s.per, most = s.block == 1024 ? 512 : s.chunks > 1 ? 1024 : 8192;
     const dim3 grid((int)(need < most ? need : most)), block(s.block);
 #define NF_FWD(C, BLOCK) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_fwd_kernel<T, C, BLOCK>), grid, block, 0, stream, xp, xs, w, \
                                             b, yp, ys, mean, rstd, rows, n, eps, s.tpr)

@@ -8,8 +8,8 @@ fp32 rounding):
   * y = xh w + b: |dy| <= h |y| + K u [(1 + max|x| r)(1 + |xh|) |w| + |b|], K = E + 30;
   * grad_x = r (u - mean u - xh mean(u xh)): two sums more, each over products with xh:
     |dgx| <= h |gx| + 4 K u r (1 + max|x| r)(1 + max|xh|)^2 max|u|;
-  * grad_w adds at most rows / 1024 + 1 terms in a thread (the grid is 1024 workgroups), 256 in a workgroup and 64 in the second
-    launch: |dgw| <= (rows / 1024 + 321 + K (1 + max|x| r)) u sum|g| (1 + |xh|), and grad_b likewise.
+  * grad_w adds at most rows / 256 + 1 terms in a thread (the grid is 256 workgroups or more), 256 in a workgroup and 64 in the
+    second launch: |dgw| <= (rows / 256 + 321 + K (1 + max|x| r)) u sum|g| (1 + |xh|), and grad_b likewise.
 """
 import pytest
 import torch
@@ -48,7 +48,7 @@ def bounds(x, w, b, g, kind, eps=1e-5):
     most = (g.double() * wd).abs().amax(-1, keepdim=True) if rows else r
     tx = h * gx.abs() + 4 * k * U * r * lift * top * most + tiny
     worst = lift.max().item() if rows else 1.0
-    chain = rows / 1024 + 321 + k * worst
+    chain = rows / 256 + 321 + k * worst
     tw = chain * U * (g.double().abs() * (1 + xh.abs())).sum(0)
     tb = chain * U * g.double().abs().sum(0)
     return (y, ty), (gx, tx), (gw, tw), (gb, tb)
