@@ -1166,7 +1166,7 @@ int next_block(const Plan& plan, bool exact, int done, int steps) {
         square += (double)g.count * g.m * g.m * g.m;
     }
     if (wide < 1.25 * square) return 1;
-    const int most = done == 0 ? (exact ? 2 : 3) : done == 3 ? 2 : 1, left = steps - done;
+    const int most = done == 0 ? (exact ? 2 : 3) : done == 3 && !exact ? 2 : 1, left = steps - done;
     return left < most ? left : most;
 }
 

@@ -169,6 +169,29 @@ def test_steps_eps_and_scale(shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('shape', [(200, 2000), (256, 1024), (1000, 384)], ids=str)
+def test_wide_fp32_keeps_the_digits_of_single_steps(shape):
+    """float32 results of wide matrices whose singular values fall over two decades: of the five steps only the first two, where
+    those are still small, may go through the smaller side at once.  Late values lie near 1 and cancel to a^-2 of the parts that
+    make them up, so a late block would lift a rounding of these parts by up to a^2 = 11.9.  The measure is the formula in torch's
+    fp32 products: they round K sums a product where the kernels round 3 K / 16, and both keep 23 to 24 bits of each matrix, so
+    step by step the kernels lose less; half as much again is allowed for the first block."""
+    gen = torch.Generator().manual_seed(5)
+    m, n = min(shape), max(shape)
+    u, v = (torch.linalg.qr(torch.randn(k, m, generator=gen, dtype=torch.float64))[0] for k in (m, n))
+    g = ((u * 10 ** (-2 * torch.arange(m) / m)) @ v.T).float().cuda()
+    g = g if shape[0] == m else g.T.contiguous()
+    want = iterate(g)
+    x = g if shape[0] == m else g.T.contiguous()
+    x = x / (x.norm() + 1e-7)
+    for _ in range(5):
+        s = x @ x.T
+        x = A * x + (B * s + C * s @ s) @ x
+    plain = norm((x if shape[0] == m else x.T) - want)
+    assert norm(nf.orthogonalize(g) - want) <= 1.5 * plain
+
+
+@pytest.mark.gpu
 def test_singular_values_come_near_one():
     g = torch.randn(96, 200, generator=torch.Generator().manual_seed(3)).cuda()
     s = torch.linalg.svdvals(nf.orthogonalize(g).double().cpu())
