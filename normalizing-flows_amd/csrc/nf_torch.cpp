@@ -1,6 +1,7 @@
 // Layer normalisation as a node of torch's autograd graph: the small calls of a conditioner are bound by the host, and a node
-// in Python costs 60 us and more a training step before any kernel runs (this one: 20 us).  The work itself is in libnf_hip.so
-// (include/nf_hip.h), whose entry points the package hands over once it has loaded that library.
+// in Python costs more than all of its kernels (256 x 64 fp32, forward + backward: 171 us, with this node 66; the forward pass
+// alone 16 and 4.5).  The work itself is in libnf_hip.so (include/nf_hip.h), whose entry points the package hands over once it
+// has loaded that library.
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -41,8 +42,7 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_de
 // rows as the entry points take them: the tensor itself, or a copy where its last axis is not contiguous (an expanded
 // gradient, a transposed view)
 Tensor unit_rows(const Tensor& t) {
-    if (t.size(1) == 1 || t.stride(1) == 1) return t;
-    return t.numel() ? t.contiguous() : at::empty(t.sizes(), t.options());
+    return t.size(1) == 1 || t.stride(1) == 1 || !t.numel() ? t : t.contiguous();
 }
 
 int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }

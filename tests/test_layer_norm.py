@@ -159,6 +159,13 @@ def test_strides_alignment_and_missing_vectors(n, start, pad, kind):
 
 
 @pytest.mark.gpu
+def test_empty_rows_of_another_stride_keep_their_graph():
+    x = torch.zeros(0, 10, device='cuda', requires_grad=True)
+    nf.layer_norm(x[:, ::2]).sum().backward()
+    assert x.grad.shape == (0, 10)
+
+
+@pytest.mark.gpu
 def test_empty_and_selected_gradients():
     w, b = torch.ones(5, device='cuda', requires_grad=True), torch.zeros(5, device='cuda', requires_grad=True)
     x = torch.zeros(0, 5, device='cuda', requires_grad=True)
