@@ -679,7 +679,7 @@ int nf_orthogonalize(const void* matrices, int64_t matrix_stride, int64_t row_st
  *   M = momentum M + grad;  U = grad + momentum M (nesterov) or M;  O = U orthogonalised as above;
  *   param = (1 - lr weight_decay) param - lr sqrt(max(1, rows / cols)) O
  * params and momenta must not overlap each other or the grads.  The workspace is that of the largest batch that one
- * sequence of launches takes (48 matrices, 8 shapes); 0 bytes mean sizes outside 1 .. 2^20. */
+ * sequence of launches takes (48 matrices, 8 shapes, 8 GiB of cells); 0 bytes mean sizes outside 1 .. 2^20. */
 size_t nf_muon_workspace_bytes(const int* rows, const int* cols, int count);
 int nf_muon_update(float* const* params, const float* const* grads, float* const* momenta, const int* rows,
                    const int* cols, int count, double lr, double momentum, int nesterov, double weight_decay, int steps,

@@ -37,6 +37,7 @@ constexpr int PIECE = 1024;              // of one term of one 32 x 16 block
 constexpr int MAX_GROUPS = 8;            // shapes in one sequence of launches
 constexpr int MAX_MATRICES = 48;         // matrices with pointers of their own (kernel arguments) in one sequence
 constexpr int NORM_BLOCKS = 256;         // partial sums of a matrix's norm
+constexpr int64_t SEQUENCE_BYTES = (int64_t)8 << 30;     // of X's and the slots' cells of one sequence of more than one matrix
 
 // matrices of one shape
 struct Group {
@@ -615,8 +616,8 @@ __global__ __launch_bounds__(256, 2) void orth_mix_kernel(Plan plan, Pointers pt
 // the polynomial) instead of three per step, everything in fp64 on its matrix instructions, whose 16 digits the recursion
 // S <- R S R, Q <- R Q (R = a + b S + c S S) cannot spend.  The norm is the trace of S.  A workgroup takes a part of the
 // columns; where there is more than one, a first launch leaves the partial sums of S and a second one adds them, iterates (in
-// every workgroup alike, 18 products of 32 x 32: 7 us) and applies.  Measured 64 us -> 12 us for 16 x 2048 against the
-// general path.
+// every workgroup alike, 19 products of 32 x 32, each waiting for the one before) and applies.  Measured against the general path:
+// 16 x 2048 35 us, there 118; 16 x 128 in one launch 24 us, there 75.
 constexpr int TINY = 32, TINY_K = 128;
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
@@ -770,7 +771,7 @@ __global__ __launch_bounds__(256) void orth_tiny_kernel(Plan plan, Pointers ptr,
 // ---- matrices that fit one workgroup's LDS ------------------------------------------------------------------------------------
 // Sides of 33 to 96 whose X, X^T and S fit it (2 SM SN + SM SM cells of 4 KB; 64 x 256 and 96 x 128 at most): one launch for
 // everything, a workgroup of eight waves per matrix with up to NC cells of X a wave.  The products are those of the general
-// path, step by step.
+// path, step by step.  Measured against it: 64 x 200 41 us, there 79; 96 x 128 41 us, there 83.
 constexpr int SMALL_CELLS = 38;          // 152 KB
 
 __device__ __forceinline__ f16x8 fragment(const char* cell, int h, int term, int lane) {
@@ -1201,9 +1202,8 @@ int64_t cut_tiny(Plan& plan) {
     return any ? doubles : 0;
 }
 
-// workspace: the tiny groups' partial sums (they are done with before the rest begins); over them partial sums of the norms, the partial accumulators of split products, then each group's X, X^T (two) and
-// slots
-// (the small ones need none)
+// workspace: the tiny groups' partial sums (they are done with before the rest begins); over them partial sums of the norms, the
+// partial accumulators of split products, then each group's X, X^T (two) and slots (the small ones need none)
 size_t layout(Plan& plan, Plan& tiny, bool exact, int64_t& partial) {
     const size_t doubles = (size_t)cut_tiny(tiny) * sizeof(double), least = doubles > 16 ? doubles : 16;
     if (!plan.groups) return least;
@@ -1219,7 +1219,8 @@ size_t layout(Plan& plan, Plan& tiny, bool exact, int64_t& partial) {
         most = floats > most ? floats : most;
     }
     at += most * sizeof(float);
-    const int block = next_block(plan, exact, 0, 3), slots = chained(plan, exact) ? SLOTS_CHAIN : block == 3 ? SLOTS_THREE : block == 2 ? SLOTS_TWO : SLOTS_ONE;
+    const int block = next_block(plan, exact, 0, 3);
+    const int slots = chained(plan, exact) ? SLOTS_CHAIN : block == 3 ? SLOTS_THREE : block == 2 ? SLOTS_TWO : SLOTS_ONE;
     for (int k = 0; k < plan.groups; ++k) {
         Group& g = plan.g[k];
         const int64_t x = (int64_t)g.count * g.sm * g.sn * CELL, s = (int64_t)g.count * g.sm * g.sm * CELL;
@@ -1486,8 +1487,12 @@ int longer(const int* shape) { return shape[0] > shape[1] ? shape[0] : shape[1];
 // Returns how many.
 int plan_muon(const int* rows, const int* cols, int from, int count, Job& job, int* order) {
     int taken = 0, shapes[MAX_GROUPS][2], groups = 0, of[MAX_MATRICES];
+    int64_t bytes = 0;
     while (from + taken < count && taken < MAX_MATRICES) {
         const int r = rows[from + taken], c = cols[from + taken];
+        const Group g = group_of(r, c, 1, 0);
+        bytes += ((int64_t)3 * g.sm * g.sn + (int64_t)SLOTS_THREE * g.sm * g.sm) * CELL;
+        if (taken && bytes > SEQUENCE_BYTES) break;
         int k = 0;
         while (k < groups && (shapes[k][0] != r || shapes[k][1] != c)) ++k;
         if (k == groups) {

@@ -11,6 +11,7 @@ moved by the roundings that the kernels make there, drawn at random:
 Independent roundings of this size give a Frobenius distance like `spread`'s; four times it is the tolerance, plus half a
 step of the result's type.  Where three and two steps go through the smaller side at once (16-bit results and the Muon step)
 the largest singular values cancel to a^-3 of the parts that make them up: 40.9 times a step's rounding 2^-24 on them is added."""
+import ctypes
 import math
 
 import pytest
@@ -125,6 +126,18 @@ def test_argument_errors_before_launch():
     assert call(g=None) == -1 and call(out=None) == -1 and call(ws=None) == -1
     assert call(ors=699) == -3 and call(oms=33 * 700 - 1) == -3 and call(g=one + 2) == -3 and call(ws=one + 8) == -3
     assert call(nbytes=need - 1) == -6
+
+
+def test_muon_workspace_is_bounded():
+    lib = nf._lib.load()
+
+    def need(count, side):
+        sides = (ctypes.c_int * count)(*[side] * count)
+        return lib.nf_muon_workspace_bytes(sides, sides, count)
+
+    # 16 matrices of 2^14 cells, eight matrices of that size each: 8 GiB; more matrices go in sequences of 16
+    assert 0 < need(1, 4096) < need(8, 4096) < need(16, 4096) == need(17, 4096) == need(200, 4096) < 9 << 30
+    assert need(1, 32768) > 8 << 30
 
 
 def test_overlap_check():
