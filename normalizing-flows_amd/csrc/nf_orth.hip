@@ -1114,26 +1114,32 @@ int cut_mix(Plan& plan, int64_t& tiles) {
 // take
 int cut_sym(Plan& plan, bool from_x, bool raw, int64_t& workgroups, int64_t& floats) {
     floats = 0;
-    int64_t work = 0, most = 0;
+    int64_t work = 0, small_work = 0, most = 0;
     for (int k = 0; k < plan.groups; ++k) plan.parts[k] = 1;
     const int64_t tiles = count_tiles(plan, 4, 4, true);
     for (int k = 0; k < plan.groups; ++k) {
         const Group& g = plan.g[k];
-        const int64_t n = (g.sm + 3) / 4, cells = from_x ? g.sn : g.sm;
+        const int64_t n = (g.sm + 3) / 4, n2 = (g.sm + 1) / 2, cells = from_x ? g.sn : g.sm;
         work += g.count * (n * (n + 1) / 2) * cells;
+        small_work += g.count * (n2 * (n2 + 1) / 2) * cells;
         most = cells > most ? cells : most;
     }
-    // a workgroup's share of the k cells, if all shares were equal and two workgroups were on each CU; at least 16 cells,
-    // whose 16 K products a partial result's 64 KB out and in cost less than
-    int64_t share = (work + 2 * CUS - 1) / (2 * CUS);
-    if (share < 16) share = 16;
+    // Small tiles where there are few large ones, or short k loops (up to 512) that leave a large tile's start and end uncovered:
+    // small ones on the same CU overlap them.
+    const bool large = tiles >= CUS / 2 && most > 16;
+    // The k cells that a CU has to go through one after the other if all were equally busy, with two large workgroups on each or
+    // a small one.  Parts pay for their second launch and a partial result's 64 KB out and in where the longest loop is 64
+    // cells more than that (800 x 4096: 236 us with parts, 248 without; 16 of 300 x 3000: 475 and 399).  A part has a workgroup's
+    // share, at least 16 cells; where that share fills the CUs, one workgroup more than fits would be another round
+    // (2000 x 4000: 1008 us with three parts, 1082 with four).
+    const int64_t even = large ? work / (2 * CUS) : small_work / CUS, share = work / (2 * CUS) > 16 ? work / (2 * CUS) : 16;
     workgroups = tiles;
-    if (raw || most >= share + share / 2) {
+    if (raw || most - even > 64) {
         workgroups = 0;
         for (int k = 0; k < plan.groups; ++k) {
             const Group& g = plan.g[k];
             const int64_t n = (g.sm + 3) / 4, cells = from_x ? g.sn : g.sm, count = g.count * (n * (n + 1) / 2);
-            const int64_t parts = cells >= share + share / 2 ? (cells + share - 1) / share : 1;
+            const int64_t parts = cells < share + share / 2 ? 1 : (raw || share == 16 ? cells + share - 1 : cells) / share;
             plan.parts[k] = (int)parts;
             plan.first_tile[k] = workgroups > 0x7fffffff ? 0x7fffffff : (int)workgroups;
             plan.partial[k] = floats;
@@ -1144,8 +1150,7 @@ int cut_sym(Plan& plan, bool from_x, bool raw, int64_t& workgroups, int64_t& flo
         plan.first_tile[plan.groups] = workgroups > 0x7fffffff ? 0x7fffffff : (int)workgroups;
         return 4;
     }
-    // short k loops (up to 512) leave a large tile's start and end uncovered: small ones on the same CU overlap them
-    if (tiles >= CUS / 2 && most > 16) return 4;
+    if (large) return 4;
     workgroups = count_tiles(plan, 2, 2, true);
     return 2;
 }
