@@ -1105,7 +1105,12 @@ constexpr int CUS = 256;
 int cut_mix(Plan& plan, int64_t& tiles) {
     // 8 x 4 cells read each operand less often, where the k loop is long enough to carry their start and end
     if ((tiles = count_tiles(plan, 8, 4, false)) >= 2 * CUS && plan.g[0].sm >= 64 && plan.groups == 1) return 8;
-    if ((tiles = count_tiles(plan, 4, 4, false)) >= CUS / 2) return 4;
+    // 4 x 4 cells against 2 x 2: k loops of up to 24 cells leave a large tile's start and end uncovered until several follow each
+    // other on a CU (300 x 3000: eight 275 us with 2 x 2, 309 with 4 x 4; 32 of 380 x 4000 1576 and 1384); longer ones carry
+    // them (1800 x 1800: 596 and 503 us)
+    int most = 0;
+    for (int k = 0; k < plan.groups; ++k) most = plan.g[k].sm > most ? plan.g[k].sm : most;
+    if ((tiles = count_tiles(plan, 4, 4, false)) >= (most <= 24 ? 4 * CUS : CUS / 2)) return 4;
     tiles = count_tiles(plan, 2, 2, false);
     return 2;
 }
