@@ -94,19 +94,43 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(Plan plan, Pointers ptr,
     if constexpr (MUON) {
         const float* gr = ptr.grad[mat];
         float* mo = ptr.momentum[mat];
-        for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)blocks * 256) {
-            const float gv = gr[e], mv = __builtin_fmaf(io.momentum, mo[e], gv);
-            mo[e] = mv;
-            const double u = io.nesterov ? __builtin_fmaf(io.momentum, mv, gv) : mv;
-            sum += u * u;
+        constexpr int EACH = 4;                          // (loads before the first store: their latency is paid once)
+        for (int64_t e0 = (int64_t)blockIdx.x * (EACH * 256) + threadIdx.x; e0 < total; e0 += (int64_t)blocks * (EACH * 256)) {
+            float gv[EACH], mv[EACH];
+#pragma unroll
+            for (int l = 0; l < EACH; ++l) {
+                const int64_t e = e0 + l * 256;
+                gv[l] = e < total ? gr[e] : 0.f;
+                mv[l] = e < total ? mo[e] : 0.f;
+            }
+#pragma unroll
+            for (int l = 0; l < EACH; ++l) {
+                const int64_t e = e0 + l * 256;
+                const float v = __builtin_fmaf(io.momentum, mv[l], gv[l]);
+                if (e < total) mo[e] = v;
+                const double u = io.nesterov ? __builtin_fmaf(io.momentum, v, gv[l]) : v;
+                sum += u * u;
+            }
         }
     } else {
         const T* in = (const T*)io.in + mat * io.in_matrix;
         const int rows = g.trans ? g.n : g.m;
-        for (int64_t row = blockIdx.x; row < rows; row += blocks)
-            for (int c = threadIdx.x; c < cols; c += 256) {
-                const double u = (double)(float)in[row * io.in_row + c];
-                sum += u * u;
+        constexpr int ROWS = 4, EACH = 4;                // (16 loads on their way)
+        for (int64_t row0 = blockIdx.x; row0 < rows; row0 += (int64_t)ROWS * blocks)
+            for (int c0 = threadIdx.x; c0 < cols; c0 += EACH * 256) {
+                float v[ROWS][EACH];
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+                    for (int l = 0; l < EACH; ++l) {
+                        const int64_t row = row0 + (int64_t)i * blocks;
+                        const int c = c0 + l * 256;
+                        v[i][l] = row < rows && c < cols ? (float)in[row * io.in_row + c] : 0.f;
+                    }
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+                    for (int l = 0; l < EACH; ++l) sum += (double)v[i][l] * v[i][l];
             }
     }
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
