@@ -164,6 +164,14 @@ def test_orthogonalize(shape, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('shape', [(130, 3000), (7000, 700), (2000, 4000), (2, 1500, 1490), (24, 390, 300), (64, 512, 500)], ids=str)
+def test_tiles_and_parts(shape):
+    """Sides at which the products take small and large tiles, whole k loops and parts of them."""
+    g = gradients(shape, 3)
+    check(nf.orthogonalize(g), g, torch.float32)
+
+
+@pytest.mark.gpu
 def test_large_matrix():
     g = gradients((2500, 3001), 5)
     check(nf.orthogonalize(g), g, torch.float32)
@@ -318,6 +326,12 @@ def test_muon_update_of_many_matrices_and_shapes():
     """More matrices (48) and shapes (8) than one sequence of launches takes."""
     check_muon([(8 + i % 11, 12) for i in range(60)], 3, lr=0.05)
     check_muon([(5, 7)] * 50, 4, lr=0.05)
+
+
+@pytest.mark.gpu
+def test_muon_update_of_long_and_short_matrices():
+    """One shape's products in parts, the others' whole, in the same launches."""
+    check_muon([(512, 300), (6000, 510), (512, 512), (90, 100), (20, 30), (512, 512)], 5, lr=0.02)
 
 
 @pytest.mark.gpu
