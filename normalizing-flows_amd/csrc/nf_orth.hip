@@ -12,7 +12,10 @@
 // products (measured beside torch's on spectra from flat to four decades), at a third of the fp16 rate instead of the
 // fp32 pipe's sixteenth.  One term is not enough even for bf16 results: five steps lift its 2^-12 to 2e-3 of the result,
 // more than the result's own rounding.  Because |X|, |S| and |b S + c S S| have spectral norms below 1.21, 1.45 and 2.81,
-// their elements times 2^15, 2^15 and 2^14 fit fp16, and lo keeps its bits down to 2^-39: fixed scales, no searches.
+// their elements times 2^15, 2^15 and 2^14 fit fp16, and lo keeps its bits down to 2^-39 of 1: fixed scales, no searches.
+// That is enough for S and b S + c S S, which stand beside the identity.  X alone can be small throughout, where |G| is far
+// below eps: its scale is 2^(15 + raise), `raise` the whole powers of two that |X| is known to lie below 1 - taken from the
+// norm for X0, less the growth of at most a factor a in every step after it (0 throughout for |G| >= eps).
 // a X is added in the epilogue, where it keeps fp32 (in the product it would cost the identity part two bits).
 //
 // Storage: a matrix is a grid of 32 x 32 cells of 4 KB, [k block of 16][term][lane][8 halfs], where lane = row + 32 (k / 8)
@@ -36,7 +39,8 @@ constexpr int CELL = 4096;               // bytes of a 32 x 32 cell
 constexpr int PIECE = 1024;              // of one term of one 32 x 16 block
 constexpr int MAX_GROUPS = 8;            // shapes in one sequence of launches
 constexpr int MAX_MATRICES = 48;         // matrices with pointers of their own (kernel arguments) in one sequence
-constexpr int NORM_BLOCKS = 256;         // partial sums of a matrix's norm
+constexpr int NORM_STRIDE = 256;         // doubles of a matrix in the workspace's first part: ...
+constexpr int NORM_BLOCKS = NORM_STRIDE - 1;             // ... partial sums of its norm, and X0's raise
 constexpr int NORM_THREADS = 512;        // of its workgroups (256: 4096 x 1024 372 us instead of 363; 1024: a Muon step of five
                                          // 256-wide layers 232 instead of 222)
 constexpr int64_t SEQUENCE_BYTES = (int64_t)8 << 30;     // of X's and the slots' cells of one sequence of more than one matrix
@@ -70,6 +74,22 @@ struct Ends {
     float momentum, keep, lr;
     int nesterov;
 };
+
+// X0's raise: 2^raise <= (norm + eps) / norm = 1 / |X0|
+__device__ __forceinline__ int raise_of(double norm, double eps) {
+    if (!(norm > 0) || !(norm + eps < INFINITY)) return 0;
+    const int e = ilogb(norm + eps) - ilogb(norm) - 1;
+    return e > 0 ? e : 0;
+}
+// ... and X's after `done` steps: a < 2^(457 / 256)
+__device__ __forceinline__ int raise_after(int first, int done) {
+    const int64_t less = ((int64_t)done * 457 + 255) >> 8;
+    return first > less ? (int)(first - less) : 0;
+}
+// where the workspace keeps it for the launches after the first two
+__device__ __forceinline__ int raise_in(const double* norms, int mat) {
+    return *reinterpret_cast<const int*>(norms + (int64_t)mat * NORM_STRIDE + NORM_BLOCKS);
+}
 
 // (LDS traffic of a wave with itself: in order, but only this tells the compiler that lanes talk to each other)
 __device__ __forceinline__ void wave_sync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -141,7 +161,7 @@ __global__ __launch_bounds__(NORM_THREADS) void orth_norm_kernel(Plan plan, Poin
     if (threadIdx.x == 0) {
         sum = 0;
         for (int w = 0; w < NORM_THREADS / 64; ++w) sum += red[w];
-        partial[(int64_t)mat * NORM_BLOCKS + blockIdx.x] = sum;
+        partial[(int64_t)mat * NORM_STRIDE + blockIdx.x] = sum;
     }
 }
 
@@ -188,7 +208,7 @@ struct Sub {
 
 // X0 in both orientations: a wave a cell
 template <typename T, bool MUON>
-__global__ __launch_bounds__(256) void orth_start_kernel(Plan plan, Pointers ptr, Ends io, const double* __restrict__ partial,
+__global__ __launch_bounds__(256) void orth_start_kernel(Plan plan, Pointers ptr, Ends io, double* partial,
                                                          int blocks, double eps, char* __restrict__ ws) {
     __shared__ uint32_t lds[4][32][33];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -201,9 +221,11 @@ __global__ __launch_bounds__(256) void orth_start_kernel(Plan plan, Pointers ptr
     if (cell >= cells) return;                           // (no barriers below: the waves are independent)
     const int mat = g.first + idx, ci = cell / g.sn, cj = cell - ci * g.sn;
     double sum = 0;
-    for (int e = lane; e < blocks; e += 64) sum += partial[(int64_t)mat * NORM_BLOCKS + e];
+    for (int e = lane; e < blocks; e += 64) sum += partial[(int64_t)mat * NORM_STRIDE + e];
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    const double scale = 32768.0 / (sqrt(sum) + eps);
+    const int raise = raise_of(sqrt(sum), eps);
+    if (cell == 0 && lane == 0) *reinterpret_cast<int*>(partial + (int64_t)mat * NORM_STRIDE + NORM_BLOCKS) = raise;
+    const double scale = ldexp(32768.0 / (sqrt(sum) + eps), raise);
     const Sub sub = {lds[wave]};
     // rows of G (cj's cells where X is its transpose)
     const int r0 = (g.trans ? cj : ci) * 32, c0 = (g.trans ? ci : cj) * 32;
@@ -250,10 +272,10 @@ __device__ __forceinline__ void piece_to_lds(const char* src, unsigned dst) {
 // the error of the whole iteration).
 constexpr int FROM_X = -1, NONE = -1;
 struct SymOp { int p, q, out, e1, e2; float k0, k1, k2; };
-struct SymOps { SymOp op[2]; };
+struct SymOps { SymOp op[2]; int done; };                // `done`: steps that X has gone through (FROM_X)
 // X <- alpha X + T X from slot r: the accumulators get scale_x * X (alpha with T's power of two), and out_scale takes them
-// back to X's scale
-struct MixOp { int r, to; float scale_x, out_scale; };
+// back to X's scale; `done` and `after`: the steps that X has gone through before and after it
+struct MixOp { int r, to; float scale_x, out_scale; int done, after; };
 
 // vmcnt(N) lgkmcnt(0): at most N loads on their way, all LDS reads back
 template <int N> __device__ __forceinline__ void wait_loads() {
@@ -452,8 +474,8 @@ __device__ __forceinline__ void triangle(int t, int n, int& ti, int& tj) {
 // Symmetric products: blockIdx.y picks the operation.  Where a group's k cells are cut into parts (or `raw`), a workgroup takes
 // one and leaves its raw accumulators in `partial`, which orth_sym_finish_kernel or orth_chain_kernel adds in order.
 template <int T, int RING>
-__global__ __launch_bounds__(256) void orth_sym_kernel(Plan plan, SymOps ops, int raw, float* __restrict__ partial,
-                                                       char* __restrict__ ws) {
+__global__ __launch_bounds__(256) void orth_sym_kernel(Plan plan, SymOps ops, int raw, const double* __restrict__ norms,
+                                                       float* __restrict__ partial, char* __restrict__ ws) {
     extern __shared__ __align__(16) char lds[];
     const SymOp& op = ops.op[blockIdx.y];
     int k = 0;
@@ -468,6 +490,7 @@ __global__ __launch_bounds__(256) void orth_sym_kernel(Plan plan, SymOps ops, in
     const int64_t slot = (int64_t)g.count * g.sm * g.sm * CELL;
     char* slots = ws + g.s + (int64_t)idx * g.sm * g.sm * CELL;
     const bool from_x = op.p == FROM_X;
+    const int raise = from_x ? raise_after(raise_in(norms, g.first + idx), ops.done) : 0;
     const char* p = from_x ? ws + g.x + (int64_t)idx * g.sm * g.sn * CELL : slots + op.p * slot;
     const char* q = from_x ? p : slots + op.q * slot;
     const int kcells = from_x ? g.sn : g.sm;
@@ -501,7 +524,7 @@ __global__ __launch_bounds__(256) void orth_sym_kernel(Plan plan, SymOps ops, in
                     *reinterpret_cast<float4*>(to + r * 256) = make_float4(ring.acc[i][j][4 * r], ring.acc[i][j][4 * r + 1],
                                                                            ring.acc[i][j][4 * r + 2], ring.acc[i][j][4 * r + 3]);
             } else {
-                finish_sym(sub, ring.acc[i][j], op.k0, slots + op.out * slot, g.sm, ci, cj, ti != tj, lane);
+                finish_sym(sub, ring.acc[i][j], ldexpf(op.k0, -2 * raise), slots + op.out * slot, g.sm, ci, cj, ti != tj, lane);
             }
         }
 }
@@ -509,8 +532,8 @@ __global__ __launch_bounds__(256) void orth_sym_kernel(Plan plan, SymOps ops, in
 // a wave a cell: the partial accumulators of a tile's parts added in order, then the cell's epilogue (plan: the groups with
 // parts only)
 template <int T>
-__global__ __launch_bounds__(256) void orth_sym_finish_kernel(Plan plan, SymOps ops, const float* __restrict__ partial,
-                                                              char* __restrict__ ws) {
+__global__ __launch_bounds__(256) void orth_sym_finish_kernel(Plan plan, SymOps ops, const double* __restrict__ norms,
+                                                              const float* __restrict__ partial, char* __restrict__ ws) {
     __shared__ uint32_t lds[4][32][33];
     const SymOp& op = ops.op[blockIdx.y];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -542,14 +565,16 @@ __global__ __launch_bounds__(256) void orth_sym_finish_kernel(Plan plan, SymOps 
     }
     const Sub sub = {lds[wave]};
     const int64_t one = (int64_t)g.sm * g.sm * CELL;
-    finish_sym(sub, acc, op.k0, ws + g.s + op.out * g.count * one + idx * one, g.sm, ci, cj, ti != tj, lane);
+    const int raise = op.p == FROM_X ? raise_after(raise_in(norms, g.first + idx), ops.done) : 0;
+    finish_sym(sub, acc, ldexpf(op.k0, -2 * raise), ws + g.s + op.out * g.count * one + idx * one, g.sm, ci, cj, ti != tj, lane);
 }
 
 enum { OUT_X, OUT_F32, OUT_BF16, OUT_F16, OUT_MUON };
 
 // X <- alpha X + T X: both orientations written (OUT_X), or the result in the caller's matrices
 template <int TI, int TJ, int RING, int OUT>
-__global__ __launch_bounds__(256, 2) void orth_mix_kernel(Plan plan, Pointers ptr, Ends io, MixOp op, char* __restrict__ ws) {
+__global__ __launch_bounds__(256, 2) void orth_mix_kernel(Plan plan, Pointers ptr, Ends io, MixOp op, const double* __restrict__ norms,
+                                                          char* __restrict__ ws) {
     extern __shared__ __align__(16) char lds[];
     int k = 0;
     while (k + 1 < plan.groups && (int)blockIdx.x >= plan.first_tile[k + 1]) ++k;
@@ -574,7 +599,11 @@ __global__ __launch_bounds__(256, 2) void orth_mix_kernel(Plan plan, Pointers pt
     ring.add(e, op.scale_x);
     const Sub sub = {reinterpret_cast<uint32_t(*)[33]>(lds + wave * 32 * 33 * 4)};
     const int rows = g.trans ? g.n : g.m, cols = g.trans ? g.m : g.n, mat = g.first + idx;
-    const float rate = OUT == OUT_MUON ? io.lr * sqrtf(fmaxf(1.f, (float)rows / (float)cols)) : 0.f;
+    // back to X's scale after the step, or to 1 - in two factors, of which one alone may lie below fp32
+    const int raise = raise_after(raise_in(norms, mat), op.done), most = raise < 64 ? raise : 64;
+    const float back = ldexpf(op.out_scale, OUT == OUT_X ? raise_after(raise_in(norms, mat), op.after) - raise : -15 - most);
+    const float rest = ldexpf(1.f, most - raise);
+    const float rate = OUT == OUT_MUON ? io.lr * sqrtf(fmaxf(1.f, (float)rows / (float)cols)) * rest : 0.f;
     // four floats of a row of the caller's matrix a lane, where its rows allow it
     float* param = OUT == OUT_MUON ? ptr.param[mat] : nullptr;
     const bool wide = OUT == OUT_MUON && (cols & 3) == 0 && ((uintptr_t)param & 15) == 0;
@@ -598,7 +627,7 @@ __global__ __launch_bounds__(256, 2) void orth_mix_kernel(Plan plan, Pointers pt
         for (int j = 0; j < FJ; ++j) {
             const int ci = ti * TI + wi * FI + i, cj = tj * TJ + wj * FJ + j;
             if (ci >= g.sm || cj >= g.sn) continue;
-            put_acc<OUT == OUT_X>(sub, lane, ring.acc[i][j], op.out_scale * (OUT == OUT_X ? 1.f : 0x1p-15f));
+            put_acc<OUT == OUT_X>(sub, lane, ring.acc[i][j], back);
             if constexpr (OUT == OUT_X) {
                 sub.store<false>(ws + g.x + xm + ((int64_t)ci * g.sn + cj) * CELL, lane);
                 sub.store<true>(ws + (op.to ? g.xt1 : g.xt0) + xm + ((int64_t)cj * g.sm + ci) * CELL, lane);
@@ -625,7 +654,8 @@ __global__ __launch_bounds__(256, 2) void orth_mix_kernel(Plan plan, Pointers pt
                 for (int it = 0; it < 16; ++it) {
                     const int r = it * 2 + (lane >> 5), c = lane & 31;
                     if (r0 + r >= rows || c0 + c >= cols) continue;
-                    const float o = __builtin_bit_cast(float, g.trans ? sub.at[c][r] : sub.at[r][c]);
+                    const float v = __builtin_bit_cast(float, g.trans ? sub.at[c][r] : sub.at[r][c]);
+                    const float o = OUT == OUT_MUON ? v : v * rest;
                     if constexpr (OUT == OUT_MUON) {
                         float* w = param + (int64_t)(r0 + r) * cols + c0 + c;
                         *w = __builtin_fmaf(-rate, o, *w * io.keep);
@@ -869,7 +899,8 @@ __device__ __forceinline__ void store_both(char* cell, char* transposed, const f
 // S comes as raw accumulators; T of alpha I + T goes to slot 0, scaled for MixOp.  Nine products of 128 x 128 take 27 us, bound by
 // the LDS, against nine launches of 5 us and more.
 template <int SM>
-__global__ __launch_bounds__(512) void orth_chain_kernel(Plan plan, int block, const float* __restrict__ partial, char* __restrict__ ws) {
+__global__ __launch_bounds__(512) void orth_chain_kernel(Plan plan, int block, int done, const double* __restrict__ norms,
+                                                         const float* __restrict__ partial, char* __restrict__ ws) {
     constexpr int SYM = (SM * (SM + 1) / 2 + 7) / 8;
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -901,6 +932,7 @@ __global__ __launch_bounds__(512) void orth_chain_kernel(Plan plan, int block, c
         return r;
     };
     Sym s;
+    const float to_s = ldexpf(1.f, -30 - 2 * raise_after(raise_in(norms, g.first + idx), done));
 #pragma unroll
     for (int u = 0; u < SYM; ++u) {
         if (ci[u] >= sm) continue;
@@ -918,7 +950,7 @@ __global__ __launch_bounds__(512) void orth_chain_kernel(Plan plan, int block, c
                 s.v[u][4 * r + 3] += v.w;
             }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s.v[u][r] *= 0x1p-30f;
+        for (int r = 0; r < 16; ++r) s.v[u][r] *= to_s;
     }
     put(p, s, 0x1p15f);
     __syncthreads();
@@ -980,6 +1012,7 @@ __global__ __launch_bounds__(512) void orth_small_kernel(Group g, Pointers ptr, 
     const T* in = MUON ? nullptr : (const T*)io.in + mat * io.in_matrix;
     const float* gr = MUON ? ptr.grad[mat] : nullptr;
     float* mo = MUON ? ptr.momentum[mat] : nullptr;
+    int raise;
     {
         float v[NC][16], gv[NC][16];
 #pragma unroll
@@ -1016,7 +1049,8 @@ __global__ __launch_bounds__(512) void orth_small_kernel(Group g, Pointers ptr, 
         __syncthreads();
         sum = 0;
         for (int w = 0; w < 8; ++w) sum += red[w];
-        const double scale = 32768.0 / (sqrt(sum) + eps);
+        raise = raise_of(sqrt(sum), eps);
+        const double scale = ldexp(32768.0 / (sqrt(sum) + eps), raise);
 #pragma unroll
         for (int t = 0; t < NC; ++t) {
             const int c = t * 8 + wave, cj = c / SM, ci = c - cj * SM;
@@ -1048,11 +1082,12 @@ __global__ __launch_bounds__(512) void orth_small_kernel(Group g, Pointers ptr, 
     const float rate = MUON ? io.lr * sqrtf(fmaxf(1.f, (float)rows / (float)cols)) : 0.f;
     for (int step = 0; step < steps; ++step) {
         f32x16 sa[SYM], xa[NC];
+        const int now = raise_after(raise, step), then = raise_after(raise, step + 1);
 #pragma unroll
         for (int u = 0; u < SYM; ++u) {
             if (si[u] >= SM) continue;
             sa[u] = cell_product(x + si[u] * g.sn * CELL, x + sj[u] * g.sn * CELL, g.sn, lane);
-            store_both(s + (si[u] * SM + sj[u]) * CELL, s + (sj[u] * SM + si[u]) * CELL, sa[u], 0x1p-15f, lane);
+            store_both(s + (si[u] * SM + sj[u]) * CELL, s + (sj[u] * SM + si[u]) * CELL, sa[u], ldexpf(1.f, -15 - 2 * now), lane);
         }
         __syncthreads();
 #pragma unroll
@@ -1080,7 +1115,7 @@ __global__ __launch_bounds__(512) void orth_small_kernel(Group g, Pointers ptr, 
             const int c = t * 8 + wave, cj = c / SM, ci = c - cj * SM;
             if (c >= cells) continue;
             if (step + 1 < steps) {
-                store_both(x + (ci * g.sn + cj) * CELL, xt + (cj * SM + ci) * CELL, xa[t], 0x1p-14f, lane);
+                store_both(x + (ci * g.sn + cj) * CELL, xt + (cj * SM + ci) * CELL, xa[t], ldexpf(1.f, -14 + then - now), lane);
                 continue;
             }
 #pragma unroll
@@ -1088,7 +1123,7 @@ __global__ __launch_bounds__(512) void orth_small_kernel(Group g, Pointers ptr, 
                 const int i = ci * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), j = cj * 32 + (lane & 31);
                 if (i >= g.m || j >= g.n) continue;
                 const int r = g.trans ? j : i, col = g.trans ? i : j;
-                const float o = xa[t][e] * 0x1p-29f;
+                const float o = ldexpf(xa[t][e], -29 - now);
                 if constexpr (MUON) {
                     float* w = ptr.param[mat] + (int64_t)r * cols + col;
                     *w = __builtin_fmaf(-rate, o, *w * io.keep);
@@ -1242,14 +1277,14 @@ int64_t cut_tiny(Plan& plan) {
     return any ? doubles : 0;
 }
 
-// workspace: the tiny groups' partial sums (they are done with before the rest begins); over them partial sums of the norms, the
+// workspace: the tiny groups' partial sums (they are done with before the rest begins); over them the norms' and raises, the
 // partial accumulators of split products, then each group's X, X^T (two) and slots (the small ones need none)
 size_t layout(Plan& plan, Plan& tiny, bool exact, int64_t& partial) {
     const size_t doubles = (size_t)cut_tiny(tiny) * sizeof(double), least = doubles > 16 ? doubles : 16;
     if (!plan.groups) return least;
     const Group& end = plan.g[plan.groups - 1];
     const int matrices = end.first + end.count;
-    int64_t at = (int64_t)matrices * NORM_BLOCKS * sizeof(double);
+    int64_t at = (int64_t)matrices * NORM_STRIDE * sizeof(double);
     partial = at;
     int64_t most = 0;
     for (int from_x = 0; from_x < 2; ++from_x) {
@@ -1294,7 +1329,7 @@ int launch_sym(const Job& job, const SymOps& ops, int count, int64_t workgroups,
     }
     float* partial = (float*)(job.ws + job.partial);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_sym_kernel<T, RING>), dim3((unsigned)workgroups, count), dim3(256), lds, job.stream,
-                       job.plan, ops, (int)raw, partial, job.ws);
+                       job.plan, ops, (int)raw, (const double*)job.ws, partial, job.ws);
     const int e = nf_launch_status();
     if (e || !parts || raw) return e;
     if constexpr (T == 4) {
@@ -1314,7 +1349,7 @@ int launch_sym(const Job& job, const SymOps& ops, int count, int64_t workgroups,
         plan.groups = groups;
         plan.first_tile[groups] = (int)total;
         hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_sym_finish_kernel<T>), dim3((unsigned)total, count), dim3(256), 0, job.stream, plan,
-                           ops, partial, job.ws);
+                           ops, (const double*)job.ws, partial, job.ws);
         return nf_launch_status();
     }
     return NF_OK;
@@ -1329,7 +1364,7 @@ int sym(Job& job, const SymOps& ops, int count, bool raw = false) {
 }
 
 template <int SM>
-int launch_chain(const Job& job, const Plan& plan, int block) {
+int launch_chain(const Job& job, const Plan& plan, int block, int done) {
     constexpr int lds = 2 * SM * SM * CELL;
     if (lds > 64 * 1024) {
         static unsigned long long done;
@@ -1337,13 +1372,13 @@ int launch_chain(const Job& job, const Plan& plan, int block) {
         if (e) return e;
     }
     hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_chain_kernel<SM>), dim3((unsigned)plan.first_tile[plan.groups]), dim3(512), lds, job.stream,
-                       plan, block, (const float*)(job.ws + job.partial), job.ws);
+                       plan, block, done, (const double*)job.ws, (const float*)(job.ws + job.partial), job.ws);
     return nf_launch_status();
 }
 
-int chain(Job& job, int block) {
+int chain(Job& job, int block, int done) {
     const SymOp op = {FROM_X, FROM_X, 0, NONE, NONE, 1.f, 0.f, 0.f};
-    int e = sym(job, SymOps{{op, op}}, 1, true);
+    int e = sym(job, SymOps{{op, op}, done}, 1, true);
     if (e) return e;
     Plan plan = job.plan;                                // a workgroup a matrix
     int64_t total = 0;
@@ -1354,10 +1389,10 @@ int chain(Job& job, int block) {
         most = plan.g[k].sm > most ? plan.g[k].sm : most;
     }
     plan.first_tile[plan.groups] = (int)total;
-    return most <= 2 ? launch_chain<2>(job, plan, block) : launch_chain<4>(job, plan, block);
+    return most <= 2 ? launch_chain<2>(job, plan, block, done) : launch_chain<4>(job, plan, block, done);
 }
 
-int sym(Job& job, SymOp op) { return sym(job, SymOps{{op, op}}, 1); }
+int sym_one(Job& job, SymOp op, int done = 0) { return sym(job, SymOps{{op, op}, done}, 1); }
 
 template <int TI, int TJ, int RING, int OUT>
 int launch_mix(const Job& job, const MixOp& op, int64_t tiles) {
@@ -1368,7 +1403,7 @@ int launch_mix(const Job& job, const MixOp& op, int64_t tiles) {
         if (e) return e;
     }
     hipLaunchKernelGGL(HIP_KERNEL_NAME(orth_mix_kernel<TI, TJ, RING, OUT>), dim3((unsigned)tiles), dim3(256), lds, job.stream, job.plan,
-                       job.ptr, job.io, op, job.ws);
+                       job.ptr, job.io, op, (const double*)job.ws, job.ws);
     return nf_launch_status();
 }
 
@@ -1476,33 +1511,35 @@ int run(Job& job) {
         const int block = next_block(plan, OUT == OUT_F32, s, job.steps);
         MixOp op;
         if (chained(plan, OUT == OUT_F32)) {
-            if ((e = chain(job, block))) return e;
+            if ((e = chain(job, block, s))) return e;
             op = block == 1 ? MixOp{0, to, CA * TWO(14), TWO(-14)}
                             : block == 2 ? MixOp{0, to, a2 * TWO(11), TWO(-11)} : MixOp{0, to, a2 * CA * TWO(9), TWO(-9)};
-            s += block;
+            op.done = s;
+            op.after = s += block;
             if ((e = s < job.steps ? mix<OUT_X>(job, op) : mix<OUT>(job, op))) return e;
             continue;
         }
-        if ((e = sym(job, {FROM_X, FROM_X, 0, NONE, NONE, TWO(-15), 0.f, 0.f}))) return e;            // S = X X^T
-        if ((e = sym(job, {0, 0, 1, 0, NONE, CC * TWO(-16), CB / CC * TWO(15), 0.f}))) return e;            // B
+        if ((e = sym_one(job, {FROM_X, FROM_X, 0, NONE, NONE, TWO(-15), 0.f, 0.f}, s))) return e;         // S = X X^T
+        if ((e = sym_one(job, {0, 0, 1, 0, NONE, CC * TWO(-16), CB / CC * TWO(15), 0.f}))) return e;            // B
         if (block == 1) {
             op = {1, to, CA * TWO(14), TWO(-14)};
         } else {
-            if ((e = sym(job, {1, 0, 2, 0, NONE, TWO(-14), CA * TWO(14), 0.f}))) return e;                       // M = a S + B S
-            if ((e = sym(job, {1, 2, 3, 2, NONE, TWO(-14), CA * TWO(14), 0.f}))) return e;                       // S' = a M + B M
-            if ((e = sym(job, {3, 3, 0, 3, NONE, CC * TWO(-16), CB / CC * TWO(15), 0.f}))) return e;        // B'
+            if ((e = sym_one(job, {1, 0, 2, 0, NONE, TWO(-14), CA * TWO(14), 0.f}))) return e;                       // M = a S + B S
+            if ((e = sym_one(job, {1, 2, 3, 2, NONE, TWO(-14), CA * TWO(14), 0.f}))) return e;                       // S' = a M + B M
+            if ((e = sym_one(job, {3, 3, 0, 3, NONE, CC * TWO(-16), CB / CC * TWO(15), 0.f}))) return e;        // B'
             const SymOps two = {{{0, 1, 2, 1, 0, TWO(-17), CA * TWO(14), CA * TWO(14)},                // T' = a B + a B' + B' B
-                                 {0, 3, 4, 3, NONE, TWO(-14), CA * TWO(14), 0.f}}};                              // M' = a S' + B' S'
+                                 {0, 3, 4, 3, NONE, TWO(-14), CA * TWO(14), 0.f}}, 0};                           // M' = a S' + B' S'
             if ((e = sym(job, two, block - 1))) return e;
             op = {2, to, a2 * TWO(11), TWO(-11)};
             if (block == 3) {
-                if ((e = sym(job, {0, 4, 1, 4, NONE, TWO(-14), CA * TWO(14), 0.f}))) return e;                   // S'' = a M' + B' M'
-                if ((e = sym(job, {1, 1, 3, 1, NONE, CC * TWO(-16), CB / CC * TWO(15), 0.f}))) return e;    // B''
-                if ((e = sym(job, {3, 2, 0, 2, 3, TWO(-16), CA * TWO(14), a2 * TWO(11)}))) return e;   // T'' = a T' + a^2 B'' + B'' T'
+                if ((e = sym_one(job, {0, 4, 1, 4, NONE, TWO(-14), CA * TWO(14), 0.f}))) return e;                   // S'' = a M' + B' M'
+                if ((e = sym_one(job, {1, 1, 3, 1, NONE, CC * TWO(-16), CB / CC * TWO(15), 0.f}))) return e;    // B''
+                if ((e = sym_one(job, {3, 2, 0, 2, 3, TWO(-16), CA * TWO(14), a2 * TWO(11)}))) return e;   // T'' = a T' + a^2 B'' + B'' T'
                 op = {0, to, a2 * CA * TWO(9), TWO(-9)};
             }
         }
-        s += block;
+        op.done = s;
+        op.after = s += block;
         if ((e = s < job.steps ? mix<OUT_X>(job, op) : mix<OUT>(job, op))) return e;
     }
     return NF_OK;

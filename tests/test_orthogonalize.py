@@ -460,3 +460,40 @@ def test_gradient_synchronizer_buckets_feed_the_step():
     muon.step()
     for p, (w, _, tol) in zip(mats, want):
         assert bool((norm(p.detach().double() - w) <= tol).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kind', TYPES, ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize('shape', [(20, 300), (70, 90), (96, 100), (150, 140), (80, 700), (256, 1024), (130, 6000), (2, 600, 9),
+                                   (500, 1100)], ids=str)
+def test_norms_far_below_eps(shape, kind):
+    """|G| << eps leaves X0 = G / (|G| + eps) small throughout; the steps lift it by a each until it is not.  Nothing in that is
+    less exact than elsewhere: the same tolerance, on every path, for the steps that stay small and for those that do not."""
+    g = gradients(shape, 1).to(kind)
+    size = norm(g).max().item()
+    for ratio, steps in ((1.0, 5), (0.1, 5), (1e-2, 5), (1e-5, 5), (1e-9, 5), (1e-12, 5), (1e-25, 5), (1e-36, 2), (1e-4, 11), (1e-12, 26)):
+        eps = size / ratio
+        check(nf.orthogonalize(g, steps=steps, eps=eps), g, kind, steps=steps, eps=eps)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shape', [(20, 300), (70, 90), (150, 140), (80, 700), (130, 6000)], ids=str)
+def test_each_matrix_has_its_own_scale(shape):
+    """One batch of norms around eps and from far above it to far below; and of zeros."""
+    g = torch.stack([gradients(shape, i, s) for i, s in enumerate((1e-3, 1e-17, 1e-10, 0.0, 1e3))])
+    out = nf.orthogonalize(g)
+    check(out, g, torch.float32)
+    assert not out[3].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shapes', [[(20, 300), (70, 90), (96, 40)], [(150, 140), (20, 300), (70, 90)], [(80, 700), (64, 64)],
+                                    [(256, 1024), (130, 6000)]], ids=str)
+def test_muon_norms_far_below_eps(shapes):
+    for eps in (1e-7, 1e2, 1e9):
+        ps, ms = ([torch.zeros(s, device='cuda') for s in shapes] for _ in range(2))
+        gs = [gradients(s, i) for i, s in enumerate(shapes)]
+        want = [muon_oracle(p, g, m, 0.5, eps=eps) for p, g, m in zip(ps, gs, ms)]
+        nf.muon_update(ps, gs, ms, lr=0.5, eps=eps)
+        for p, (w, _, tol) in zip(ps, want):
+            assert bool((norm(p.double() - w) <= tol).all()), (eps, p.shape)
