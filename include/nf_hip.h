@@ -665,7 +665,7 @@ int nf_layer_norm_bwd(const void* grad_y, int64_t grad_y_row_stride, const void*
  * G (rows x cols) -> X with the singular vectors of G and singular values near 1, by `steps` Newton-Schulz products:
  *   X = G / (|G|_F + eps);  steps times  S = X X^T, X = a X + (b S + c S S) X,  a, b, c = 3.4445, -4.7750, 2.0315
  * on the smaller side (rows > cols: on G^T).  Products of fp32 accuracy on the fp16 matrix pipe; the norm in fp64.  A zero
- * matrix gives zeros; a NaN or infinity anywhere in a matrix makes all of that matrix NaN, and no other. */
+ * matrix gives zeros (with eps = 0 NaN); a NaN or infinity anywhere in a matrix makes all of that matrix NaN, and no other. */
 
 /* Bytes of the caller-owned workspace (16-byte aligned); 0 for count = 0, an unknown type or sizes outside 1 .. 2^20 (count: 65535). */
 size_t nf_orthogonalize_workspace_bytes(int64_t count, int rows, int cols, int elem);

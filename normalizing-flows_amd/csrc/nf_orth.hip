@@ -75,6 +75,11 @@ struct Ends {
     int nesterov;
 };
 
+// 1 / (norm + eps), finite for a zero matrix over the smallest eps too (zeros stay zeros; with eps = 0 they are NaN)
+__device__ __forceinline__ double over_norm(double norm, double eps) {
+    const double d = norm + eps;
+    return 1.0 / (d > 0 && d < 1e-290 ? 1e-290 : d);
+}
 // X0's raise: 2^raise <= (norm + eps) / norm = 1 / |X0|
 __device__ __forceinline__ int raise_of(double norm, double eps) {
     if (!(norm > 0) || !(norm + eps < INFINITY)) return 0;
@@ -225,7 +230,7 @@ __global__ __launch_bounds__(256) void orth_start_kernel(Plan plan, Pointers ptr
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
     const int raise = raise_of(sqrt(sum), eps);
     if (cell == 0 && lane == 0) *reinterpret_cast<int*>(partial + (int64_t)mat * NORM_STRIDE + NORM_BLOCKS) = raise;
-    const double scale = ldexp(32768.0 / (sqrt(sum) + eps), raise);
+    const double scale = ldexp(over_norm(sqrt(sum), eps), raise + 15);
     const Sub sub = {lds[wave]};
     // rows of G (cj's cells where X is its transpose)
     const int r0 = (g.trans ? cj : ci) * 32, c0 = (g.trans ? ci : cj) * 32;
@@ -769,10 +774,10 @@ __global__ __launch_bounds__(256) void orth_tiny_kernel(Plan plan, Pointers ptr,
     __syncthreads();
     double trace = 0;
     for (int i = 0; i < TINY; ++i) trace += s[i][i];
-    const double scale = 1.0 / (sqrt(trace) + eps);
+    const double scale = over_norm(sqrt(trace), eps);
     __syncthreads();
     for (int e = threadIdx.x; e < TINY * TINY; e += 256) {
-        s[e >> 5][e & 31] *= scale * scale;
+        s[e >> 5][e & 31] = s[e >> 5][e & 31] * scale * scale;
         q[e >> 5][e & 31] = (e >> 5) == (e & 31);
     }
     __syncthreads();
@@ -1050,7 +1055,7 @@ __global__ __launch_bounds__(512) void orth_small_kernel(Group g, Pointers ptr, 
         sum = 0;
         for (int w = 0; w < 8; ++w) sum += red[w];
         raise = raise_of(sqrt(sum), eps);
-        const double scale = ldexp(32768.0 / (sqrt(sum) + eps), raise);
+        const double scale = ldexp(over_norm(sqrt(sum), eps), raise + 15);
 #pragma unroll
         for (int t = 0; t < NC; ++t) {
             const int c = t * 8 + wave, cj = c / SM, ci = c - cj * SM;

@@ -497,3 +497,15 @@ def test_muon_norms_far_below_eps(shapes):
         nf.muon_update(ps, gs, ms, lr=0.5, eps=eps)
         for p, (w, _, tol) in zip(ps, want):
             assert bool((norm(p.double() - w) <= tol).all()), (eps, p.shape)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shape', [(20, 70), (20, 700), (40, 70), (130, 150), (70, 900)], ids=str)
+def test_zeros_over_the_smallest_eps(shape):
+    """0 / (0 + eps) = 0 where eps, its reciprocal or that one's square leave the range of float64; 0 / 0 is NaN."""
+    g = torch.zeros(shape, device='cuda')
+    for eps in (1e-7, 1e-160, 1e-300, 1e-310, 5e-324):
+        assert torch.equal(nf.orthogonalize(g, eps=eps), g)
+    assert nf.orthogonalize(g, eps=0.0).isnan().all()
+    h = gradients(shape, 1)
+    assert torch.equal(nf.orthogonalize(h, eps=5e-324), nf.orthogonalize(h, eps=0.0))
