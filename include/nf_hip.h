@@ -667,7 +667,7 @@ int nf_layer_norm_bwd(const void* grad_y, int64_t grad_y_row_stride, const void*
  * on the smaller side (rows > cols: on G^T).  Products of fp32 accuracy on the fp16 matrix pipe; the norm in fp64.  A zero
  * matrix gives zeros (with eps = 0 NaN); a NaN or infinity anywhere in a matrix makes all of that matrix NaN, and no other. */
 
-/* Bytes of the caller-owned workspace (16-byte aligned); 0 for count = 0, an unknown type or sizes outside 1 .. 2^20 (count: 65535). */
+/* Bytes of the caller-owned workspace (16-byte aligned), which do for every smaller count too; 0 for count = 0, an unknown type or sizes outside 1 .. 2^20 (count: 65535). */
 size_t nf_orthogonalize_workspace_bytes(int64_t count, int rows, int cols, int elem);
 /* `count` matrices of type `elem`, matrix i at matrices + i * matrix_stride with contiguous rows row_stride apart (strides
  * in elements; an input's may be 0).  out: the same type, another buffer than `matrices`. */

@@ -1251,6 +1251,29 @@ int next_block(const Plan& plan, bool exact, int done, int steps) {
     return left < most ? left : most;
 }
 
+// The floats of cut_sym's parts do not grow with the count of matrices (more of them are cut into fewer parts), but a
+// workspace for a count has to do for every smaller one.  This many do, for one group: t tiles of one matrix, at most `parts` a
+// tile, and while a share is 16 cells (count t cells < 17 * 512) count t parts <= 17 * 512 parts / cells; larger shares make
+// fewer parts, 512 * 18 / 17 and, where the last one of a tile may be short (raw), one a matrix more.
+int64_t most_floats(const Plan& plan, bool from_x, bool raw) {
+    const Group& g = plan.g[0];
+    const int64_t n = (g.sm + 3) / 4, t = n * (n + 1) / 2, cells = from_x ? g.sn : g.sm;
+    const int64_t parts = cells < 24 ? 1 : (cells + 15) / 16, all = g.count * t * parts;
+    if (raw) return (all < 544 + g.count ? all : 544 + g.count) * 16 * 1024;
+    // (whether there are any: the even share grows with the count but where tiles become large)
+    const int64_t change = (CUS / 2 + t - 1) / t;
+    bool any = false;
+    for (const int64_t count : {(int64_t)1, change < g.count ? change : g.count}) {
+        Plan some = plan;
+        some.g[0].count = (int)count;
+        int64_t workgroups, floats;
+        cut_sym(some, from_x, false, workgroups, floats);
+        any = any || floats;
+    }
+    const int64_t most = (17 * 512 - 1) * parts / cells;
+    return any ? 2 * (all < most ? all : most) * 16 * 1024 : 0;
+}
+
 constexpr int SLOTS_CHAIN = 1, SLOTS_ONE = 2, SLOTS_TWO = 4, SLOTS_THREE = 5;
 
 // Whether the m x m side is orth_chain_kernel's: all its matrices within 4 x 4 cells, and blocks of steps to save launches in
@@ -1295,7 +1318,8 @@ size_t layout(Plan& plan, Plan& tiny, bool exact, int64_t& partial) {
     for (int from_x = 0; from_x < 2; ++from_x) {
         int64_t workgroups, floats;
         if (chained(plan, exact) && !from_x) continue;
-        cut_sym(plan, from_x, chained(plan, exact), workgroups, floats);
+        if (plan.groups == 1) floats = most_floats(plan, from_x, chained(plan, exact));
+        else cut_sym(plan, from_x, chained(plan, exact), workgroups, floats);
         most = floats > most ? floats : most;
     }
     at += most * sizeof(float);

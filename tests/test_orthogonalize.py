@@ -509,3 +509,24 @@ def test_zeros_over_the_smallest_eps(shape):
     assert nf.orthogonalize(g, eps=0.0).isnan().all()
     h = gradients(shape, 1)
     assert torch.equal(nf.orthogonalize(h, eps=5e-324), nf.orthogonalize(h, eps=0.0))
+
+
+@pytest.mark.parametrize('elem', [0, 1])
+@pytest.mark.parametrize('rows,cols,counts', [(33, 32544, (254, 255, 256, 257, 300)), (64, 27936, (300, 340, 341, 342, 400)),
+                                              (300, 3000, range(1, 60)), (100, 3000, range(1, 700, 7)), (4096, 4096, (1, 2, 3, 4)),
+                                              (2500, 700, range(1, 80)), (20, 9000, range(1, 9))])
+def test_a_workspace_does_for_every_smaller_count(rows, cols, counts, elem):
+    """More matrices are cut into fewer parts of their k loops, so what the parts take does not grow with the count; the answer
+    has to, since a batch that is cut ends with a smaller part."""
+    lib = nf._lib.load()
+    need = [lib.nf_orthogonalize_workspace_bytes(n, rows, cols, elem) for n in counts]
+    assert need[0] > 0 and all(a <= b for a, b in zip(need, need[1:]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shape,per', [((11, 300, 3000), 6), ((7, 130, 3000), 3), ((5, 20, 3000), 2), ((9, 100, 3000), 4)], ids=str)
+def test_a_cut_batch_of_matrices_in_parts(shape, per, monkeypatch):
+    """A shorter last part, whose k loops are cut into more parts than the others'."""
+    g = gradients(shape, 6)
+    monkeypatch.setattr(nf._lib, 'WORKSPACE_BYTES', per * nf._lib.load().nf_orthogonalize_workspace_bytes(1, *shape[1:], 0))
+    check(nf.orthogonalize(g), g, torch.float32)
