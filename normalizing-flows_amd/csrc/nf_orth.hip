@@ -1235,9 +1235,9 @@ int cut_sym(Plan& plan, bool from_x, bool raw, int64_t& workgroups, int64_t& flo
 // over X, 3 m^2 n flop each.  The price is digits: the identity part alpha = a^j of the block's product cancels most of the
 // largest singular values (their factor is near a^-j of it).  Frobenius errors measured against 64 bits, m >= 64, spectra
 // from flat to four decades: 1.3e-6 to 5.9e-6 step by step (fp32 products: 1.3e-6 to 5.1e-6), at most 1.2 times that with
-// two steps first, 2e-6 to 7.5e-6 with three and two.  So fp32 results get the first; 16-bit results, whose own rounding is
-// 2e-4 and more, and the Muon step, whose parameters keep 1e-7 of it, the second.  Below m = 64 (few rounding errors to
-// average) and where X is not wide, step by step.
+// two steps first, 2e-6 to 7.5e-6 with three and two.  So fp32 results and the Muon step (`exact`) get the first, 16-bit
+// results, whose own rounding is 2e-4 and more, the second.  Below m = 64 (few rounding errors to average) and where X is not
+// wide, step by step.
 int next_block(const Plan& plan, bool exact, int done, int steps) {
     double wide = 0, square = 0;
     for (int k = 0; k < plan.groups; ++k) {
@@ -1536,10 +1536,11 @@ int run(Job& job) {
                        job.io, partial, (int)blocks, job.eps, job.ws);
     if ((e = nf_launch_status())) return e;
     const float a2 = CA * CA;
+    constexpr bool exact = OUT != OUT_BF16 && OUT != OUT_F16;
     for (int s = 0, to = 1; s < job.steps; to ^= 1) {
-        const int block = next_block(plan, OUT == OUT_F32, s, job.steps);
+        const int block = next_block(plan, exact, s, job.steps);
         MixOp op;
-        if (chained(plan, OUT == OUT_F32)) {
+        if (chained(plan, exact)) {
             if ((e = chain(job, block, s))) return e;
             op = block == 1 ? MixOp{0, to, CA * TWO(14), TWO(-14)}
                             : block == 2 ? MixOp{0, to, a2 * TWO(11), TWO(-11)} : MixOp{0, to, a2 * CA * TWO(9), TWO(-9)};
@@ -1597,7 +1598,7 @@ int plan_muon(const int* rows, const int* cols, int from, int count, Job& job, i
     while (from + taken < count && taken < MAX_MATRICES) {
         const int r = rows[from + taken], c = cols[from + taken];
         const Group g = group_of(r, c, 1, 0);
-        bytes += ((int64_t)3 * g.sm * g.sn + (int64_t)SLOTS_THREE * g.sm * g.sm) * CELL;
+        bytes += ((int64_t)3 * g.sm * g.sn + (int64_t)SLOTS_THREE * g.sm * g.sm) * CELL;      // (at least what layout gives it)
         if (taken && bytes > SEQUENCE_BYTES) break;
         int k = 0;
         while (k < groups && (shapes[k][0] != r || shapes[k][1] != c)) ++k;
@@ -1691,7 +1692,7 @@ extern "C" size_t nf_muon_workspace_bytes(const int* rows, const int* cols, int 
             if (!sizes_ok(1, rows[i], cols[i])) return 0;
         Job job = {};
         const int taken = plan_muon(rows, cols, at, count, job, order);
-        const size_t need = layout(job.plan, job.tiny, false, job.partial);
+        const size_t need = layout(job.plan, job.tiny, true, job.partial);
         most = need > most ? need : most;
         at += taken;
     }
@@ -1715,7 +1716,7 @@ extern "C" int nf_muon_update(float* const* params, const float* const* grads, f
     for (int at = 0; at < count;) {
         Job job = {};
         const int taken = plan_muon(rows, cols, at, count, job, order);
-        layout(job.plan, job.tiny, false, job.partial);
+        layout(job.plan, job.tiny, true, job.partial);
         for (int i = 0; i < taken; ++i) {
             job.ptr.grad[i] = grads[order[i]];
             job.ptr.momentum[i] = momenta[order[i]];

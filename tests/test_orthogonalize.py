@@ -530,3 +530,45 @@ def test_a_cut_batch_of_matrices_in_parts(shape, per, monkeypatch):
     g = gradients(shape, 6)
     monkeypatch.setattr(nf._lib, 'WORKSPACE_BYTES', per * nf._lib.load().nf_orthogonalize_workspace_bytes(1, *shape[1:], 0))
     check(nf.orthogonalize(g), g, torch.float32)
+
+
+def plain_update(u, eps=1e-7):
+    """The update in torch's fp32 products, step by step."""
+    x = u if u.shape[0] <= u.shape[1] else u.T.contiguous()
+    x = x / (x.norm() + eps)
+    for _ in range(5):
+        s = x @ x.T
+        x = A * x + (B * s + C * s @ s) @ x
+    return x if u.shape[0] <= u.shape[1] else x.T
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('decades', [0, 2, 4])
+@pytest.mark.parametrize('shapes', [[(200, 2000)], [(1000, 384)], [(64, 128)], [(128, 700), (128, 128)],
+                                    [(512, 784), (512, 512), (512, 512), (4000, 512)], [(128, 64), (128, 128), (1472, 128)]], ids=str)
+def test_muon_keeps_the_digits_of_single_steps(shapes, decades):
+    """The Muon step of parameters that start at zero is the update alone: as exact as a float32 result of nf.orthogonalize, by
+    the measure of test_wide_fp32_keeps_the_digits_of_single_steps (torch's fp32 products, half as much again), over the step's
+    matrices together.
+
+    That measure alone does not hold for equal singular values (decades = 0): S is then a multiple of the identity, K squares
+    of one sign, which the kernels sum in 3 K / 16 fp32 additions one after the other - at K = 2000 an error of
+    0.58 * 2^-24 sqrt(3 * 2000 / 16 + 16) = 6.8e-7 of S, by the model above - and a library that adds its K in several sums
+    that it joins does not have it (its whole error there is 3.4e-7).  So there `spread`, what the model's roundings of single steps
+    come to, is added."""
+    gen = torch.Generator().manual_seed(8)
+    gs = []
+    for m, n in shapes:
+        k = min(m, n)
+        u, v = (torch.linalg.qr(torch.randn(d, k, generator=gen, dtype=torch.float64))[0] for d in (m, n))
+        gs.append(((u * 10 ** (-decades * torch.arange(k) / k)) @ v.T).float().cuda())
+    ps, ms = ([torch.zeros(s, device='cuda') for s in shapes] for _ in range(2))
+    nf.muon_update(ps, gs, ms, lr=1.0, momentum=0.0)
+    sums = [0.0, 0.0, 0.0]
+    for p, g in zip(ps, gs):
+        want, rate = iterate(g), math.sqrt(max(1, g.shape[0] / g.shape[1]))
+        model = iterate(g, gen=torch.Generator(device='cuda').manual_seed(77))
+        for i, e in enumerate((-p - rate * want, rate * (plain_update(g) - want), rate * (model - want))):
+            sums[i] += norm(e).item() ** 2
+    ours, plain, spread = (math.sqrt(v) for v in sums)
+    assert ours <= 1.5 * plain + (spread if decades == 0 else 0), (ours, plain, spread)
