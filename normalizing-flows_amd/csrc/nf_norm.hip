@@ -198,8 +198,10 @@ __global__ __launch_bounds__(BLOCK) void norm_fwd_kernel(const T* __restrict__ x
 }
 
 // partial: [gridDim.x][2][n] (grad_w, then grad_b), each the workgroup's rows; dynamic LDS: (rows at a time) * n
-// floats where a workgroup handles several rows at a time
-template <typename T, int C, int BLOCK>
+// floats where a workgroup handles several rows at a time.  RAGGED: the row ends inside a chunk.  What lies past its end is
+// left out by g = 0 there - and by a condition an element, since 0 times (0 - mu) r is NaN where the latter leaves fp32.  Rows of
+// whole chunks are spared it (16384 x 16384 bf16, forward + backward: 608 us, with it 635; 16384 x 12001, which needs it: 744 us).
+template <typename T, int C, int BLOCK, bool RAGGED>
 __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(const T* __restrict__ g, int64_t gs, const T* __restrict__ x,
                                                         int64_t xs, const float* __restrict__ mean,
                                                         const float* __restrict__ rstd, const float* __restrict__ w,
@@ -250,8 +252,8 @@ __global__ __launch_bounds__(BLOCK) void norm_bwd_kernel(const T* __restrict__ g
             widen<T>(ahead_g[c], gv[c]);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                xh[c][e] = live && col < n ? (xh[c][e] - mu) * r : 0.f;
-                const float u = gv[c][e] * wv[c][e];     // (past the row's end g is 0: nothing is added)
+                xh[c][e] = live && col + (RAGGED ? e : 0) < n ? (xh[c][e] - mu) * r : 0.f;
+                const float u = gv[c][e] * wv[c][e];
                 s1 += u;
                 s2 = __builtin_fmaf(u, xh[c][e], s2);
                 aw[c][e] = __builtin_fmaf(gv[c][e], xh[c][e], aw[c][e]);
@@ -506,14 +508,17 @@ int launch_bwd(const void* g, int64_t gs, const void* x, int64_t xs, const float
         const dim3 grid(count), block(s.block);
         const size_t lds = (sums && s.per > 1) ? (size_t)s.per * n * sizeof(float) : 0;
         float* to = sums ? partial : nullptr;
-#define NF_BWD(C, BLOCK) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_bwd_kernel<T, C, BLOCK>), grid, block, lds, stream, gp, gs, \
-                                            xp, xs, mean, rstd, w, gxp, gxs, to, rows, n, s.tpr)
+        const bool ragged = n % Chunk<T>::V != 0;
+#define NF_GO(C, BLOCK, RAGGED) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_bwd_kernel<T, C, BLOCK, RAGGED>), grid, block, lds, stream, \
+                                                   gp, gs, xp, xs, mean, rstd, w, gxp, gxs, to, rows, n, s.tpr)
+#define NF_BWD(C, BLOCK) do { if (ragged) NF_GO(C, BLOCK, true); else NF_GO(C, BLOCK, false); } while (0)
         if (s.block == 1024) NF_BWD(EMAX_WIDE / Chunk<T>::V, 1024);
         else if (s.chunks == 1) NF_BWD(1, 256);
         else if (s.chunks == 2) NF_BWD(2, 256);
         else if (s.chunks == 4) NF_BWD(4, 256);
         else if constexpr (Chunk<T>::V == 4) NF_BWD(8, 256);
 #undef NF_BWD
+#undef NF_GO
     }
     int e = nf_launch_status();
     if (e || !sums) return e;

@@ -367,3 +367,27 @@ def test_coupling_flow_with_layer_norm_is_invertible():
     loss.backward()
     norms = [m for m in flow.modules() if isinstance(m, nf.LayerNorm)]
     assert len(norms) == 8 and all(m.weight.grad is not None and m.weight.grad.isfinite().all() for m in norms)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kind', [torch.float32, torch.bfloat16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize('n', [3, 5, 37, 40, 130, 515, 1031, 2050, 8193, 16386])
+def test_constant_rows_of_the_largest_values(n, kind):
+    """x - mu = 0 in rows of one value (a power of two, which no sum rounds), so xh = 0, y = b, grad_w = 0, grad_b = sum g and
+    grad_x = r (u - mean u) with r = 1 / sqrt(eps), however large the value is: nothing of what lies past a row's end gets in,
+    where (0 - mu) r leaves fp32 (2^110 * 10^6)."""
+    _, w, b, g = data(6, n, kind, n)
+    x = torch.full((6, n), 2.0 ** 110).to(kind)
+    x[3:] *= -1
+    xd, wd, bd = x.cuda().requires_grad_(), w.cuda().requires_grad_(), b.cuda().requires_grad_()
+    y = nf.layer_norm(xd, wd, bd, eps=1e-12)
+    gx, gw, gb = (t.cpu() for t in torch.autograd.grad(y, (xd, wd, bd), g.cuda()))
+    h = torch.finfo(kind).eps / 2
+    assert torch.equal(y.detach().cpu(), b.to(kind).expand(6, n))
+    assert not gw.any()
+    # (sums of at most 16384 / 1024 + 22 additions a thread and between threads, those of six rows and two launches)
+    k = 62
+    u = g.double() * w.double()
+    want, r = u - u.mean(-1, keepdim=True), 1e6
+    assert bool(((gx.double() - want * r).abs() <= h * r * want.abs() + 4 * k * U * r * u.abs().amax(-1, keepdim=True)).all())
+    assert bool(((gb.double() - g.double().sum(0)).abs() <= 321 * U * g.double().abs().sum(0)).all())
