@@ -114,6 +114,11 @@ std::optional<Tensor> vector(const std::optional<Tensor>& t, const char* name, c
     return t->contiguous();
 }
 
+// (a tangent of forward-mode differentiation would be dropped without a word)
+void check_tangent(const Tensor& t, const char* name) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "layer_norm has no forward-mode derivative: ", name, " carries a tangent");
+}
+
 // A leaf whose gradient an earlier graph, still alive, accumulates on another stream: a backward pass captured with it would
 // wait for that stream from inside the capture, which ends the process.  Refused here, before anything is recorded.
 void check_capture(const Tensor& t, const char* name) {
@@ -136,6 +141,9 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
                       "x must have a last axis of at least one element, got shape ", x.sizes());
     TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "eps must be a finite number >= 0, got ", eps);
     const auto w = vector(weight, "weight", x), b = vector(bias, "bias", x);
+    check_tangent(x, "x");
+    if (w) check_tangent(*w, "weight");
+    if (b) check_tangent(*b, "bias");
     const Tensor rows = unit_rows(x.dim() == 2 ? x : x.reshape({-1, x.size(-1)}));
     const bool records = at::GradMode::is_enabled() && (x.requires_grad() || (w && w->requires_grad()) ||
                                                         (b && b->requires_grad()));

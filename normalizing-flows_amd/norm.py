@@ -16,8 +16,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (biased variance; statistics in fp32).
 
     x: [..., features] on the GPU, float32, bfloat16 or float16, rows at any stride; the result has its shape and type.
-    weight, bias: float32 vectors of `features` elements, or None.  Differentiable once (not under create_graph) in x, weight
-    and bias; the gradients of weight and bias are summed in a fixed order (the same inputs give the same bits)."""
+    weight, bias: float32 vectors of `features` elements, or None.  eps >= 0 is taken as float32.  Differentiable once, by
+    backward passes (not under create_graph, nor in forward mode), in x, weight and bias; the gradients of weight and bias are
+    summed in a fixed order (the same inputs give the same bits)."""
     return _lib.nodes().layer_norm(x, weight, bias, eps)
 
 

@@ -13,6 +13,7 @@ import math
 import numbers
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -28,13 +29,21 @@ def _check_number(name, value, low, below=math.inf):
         raise ValueError('%s must be a number in [%g, %g), got %r' % (name, low, below, value))
 
 
+def _check_tangents(name, tensors):
+    """A tangent of forward-mode differentiation would be dropped without a word."""
+    if getattr(forward_ad, '_current_level', 0) < 0:    # (outside any: a step's 90 tensors would take 40 us)
+        return
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError('%s carry a tangent: there is no forward-mode derivative' % name)
+
+
 def orthogonalize(matrices, steps=5, eps=1e-7):
     """X = G / (|G|_F + eps), then `steps` times X <- a X + (b S + c S S) X with S = X X^T and a, b, c = 3.4445, -4.7750,
     2.0315 (on G^T where G has more rows than columns): each singular value s goes through the odd quintic
     a s + b s^3 + c s^5, which brings all but the smallest near 1 (0.7 to 1.2) and leaves the singular vectors.
 
     matrices: [..., rows, cols] on the GPU, float32, bfloat16 or float16, any strides; the result has its shape and type.
-    Computed to fp32 accuracy.  Not differentiable."""
+    Computed to fp32 accuracy.  Not differentiable, in no mode."""
     if not isinstance(matrices, torch.Tensor) or not matrices.is_cuda:
         raise RuntimeError('matrices must be a tensor on the GPU (MI355X); this package has no CPU path')
     if matrices.dtype not in _lib.NF_ELEM:
@@ -43,6 +52,7 @@ def orthogonalize(matrices, steps=5, eps=1e-7):
         raise ValueError('matrices must be [..., rows, cols] with sides of 1 to %d, got shape %s'
                          % (_lib.MAX_SIDE, tuple(matrices.shape)))
     _check_iteration(steps, eps)
+    _check_tangents('matrices', [matrices])
     if torch.is_grad_enabled() and matrices.requires_grad:
         raise NotImplementedError('orthogonalize has no backward kernel: call under torch.no_grad() or detach()')
     g = matrices.detach().reshape(-1, *matrices.shape[-2:])
@@ -102,6 +112,7 @@ def muon_update(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=Tru
     _check_matrices('params', params, shapes, device, True)
     _check_matrices('grads', grads, shapes, device, False)
     _check_matrices('momentum_buffers', momenta, shapes, device, True)
+    _check_tangents('params, grads or momentum_buffers', params + grads + momenta)
     some = [i for i, s in enumerate(shapes) if s[0] and s[1]]
     if len(some) < len(params):
         params, grads, momenta = ([ts[i] for i in some] for ts in (params, grads, momenta))

@@ -391,3 +391,21 @@ def test_constant_rows_of_the_largest_values(n, kind):
     want, r = u - u.mean(-1, keepdim=True), 1e6
     assert bool(((gx.double() - want * r).abs() <= h * r * want.abs() + 4 * k * U * r * u.abs().amax(-1, keepdim=True)).all())
     assert bool(((gb.double() - g.double().sum(0)).abs() <= 321 * U * g.double().abs().sum(0)).all())
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    """A tangent is not dropped, whether or not its tensor requires a gradient; other tensors pass inside a dual level too."""
+    from torch.autograd import forward_ad
+    x, w, b = torch.randn(5, 8, device='cuda'), torch.ones(8, device='cuda'), torch.zeros(8, device='cuda')
+    want = nf.layer_norm(x, w, b)
+    with forward_ad.dual_level():
+        assert torch.equal(nf.layer_norm(x, w, b), want)
+        for at in range(3):
+            for grad in (False, True):
+                args = [t.clone().requires_grad_(grad) for t in (x, w, b)]
+                args[at] = forward_ad.make_dual(args[at], torch.ones_like(args[at]))
+                with pytest.raises(NotImplementedError, match='tangent'):
+                    nf.layer_norm(*args)
+                with torch.no_grad(), pytest.raises(NotImplementedError, match='tangent'):
+                    nf.layer_norm(*args)

@@ -572,3 +572,20 @@ def test_muon_keeps_the_digits_of_single_steps(shapes, decades):
             sums[i] += norm(e).item() ** 2
     ours, plain, spread = (math.sqrt(v) for v in sums)
     assert ours <= 1.5 * plain + (spread if decades == 0 else 0), (ours, plain, spread)
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad
+    g = gradients((6, 9), 1)
+    p, m = torch.zeros_like(g), torch.zeros_like(g)
+    want = nf.orthogonalize(g)
+    with forward_ad.dual_level():
+        assert torch.equal(nf.orthogonalize(g), want)
+        dual = forward_ad.make_dual(g, torch.ones_like(g))
+        with pytest.raises(NotImplementedError, match='tangent'):
+            nf.orthogonalize(dual)
+        for args in (([p], [dual], [m]), ([dual], [p], [m]), ([p], [m], [dual])):
+            with pytest.raises(NotImplementedError, match='tangent'):
+                nf.muon_update(*args, lr=0.1)
+    assert not p.any() and not m.any()
