@@ -119,16 +119,19 @@ void check_tangent(const Tensor& t, const char* name) {
     TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "layer_norm has no forward-mode derivative: ", name, " carries a tangent");
 }
 
-// A leaf whose gradient an earlier graph, still alive, accumulates on another stream: a backward pass captured with it would
-// wait for that stream from inside the capture, which ends the process.  Refused here, before anything is recorded.
+// A leaf whose gradient an earlier graph, still alive, accumulates on the default stream: a backward pass captured with it would
+// make that stream wait for the captured one, which no capture allows and which ends the process.  Refused here, before anything
+// is recorded.  (Any other stream joins the capture and is joined again at the pass's end: a warm-up on a side stream may keep its
+// outputs, hooks may hold an accumulator made there.)
 void check_capture(const Tensor& t, const char* name) {
     if (!t.is_leaf() || !t.requires_grad()) return;
     const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
     if (!accumulator) return;
     const auto stream = accumulator->stream();
-    TORCH_CHECK(!stream || stream->id() == c10::hip::getCurrentHIPStream(t.get_device()).id(), name,
-                " takes part in an autograd graph that was recorded on another stream and is still alive: delete that graph's "
-                "outputs before capturing a training step");
+    TORCH_CHECK(!stream || *stream != c10::Stream(c10::Stream::DEFAULT, t.device()), name,
+                " takes part in an autograd graph that was recorded on the default stream and is still alive (or a hook holds its "
+                "gradient accumulator): before capturing a training step, delete that graph's outputs, or record it and make the "
+                "hooks under torch.cuda.stream(a side stream)");
 }
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {

@@ -409,3 +409,41 @@ def test_forward_mode_is_refused():
                     nf.layer_norm(*args)
                 with torch.no_grad(), pytest.raises(NotImplementedError, match='tangent'):
                     nf.layer_norm(*args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('held', ['outputs', 'accumulators'])
+def test_capture_after_a_warm_up_whose_graph_lives(held):
+    """The usual recipe: warm up on a side stream, then capture.  What the warm-up left alive - its outputs, or the gradient
+    accumulators that hooks hold for good - belongs to a stream that can join the capture, so the captured step, whose gradients
+    that stream accumulates, gives the eager one's values at every replay."""
+    n = 72
+    m, x, g = nf.LayerNorm(n).cuda(), torch.zeros(50, n, device='cuda'), torch.zeros(50, n, device='cuda')
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = m(x)
+        if held == 'accumulators':
+            alive.backward(g)
+            alive = [p.expand_as(p).grad_fn.next_functions[0][0] for p in m.parameters()]
+    torch.cuda.current_stream().wait_stream(side)
+    for p in m.parameters():
+        p.grad = torch.ones_like(p)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for p in m.parameters():
+            p.grad.zero_()
+        m(x).backward(g)
+    other = nf.LayerNorm(n).cuda()
+    for seed in range(4):
+        xs, w, b, gs = data(50, n, torch.float32, seed)
+        with torch.no_grad():
+            for t, v in ((x, xs), (g, gs), (m.weight, w), (m.bias, b), (other.weight, w), (other.bias, b)):
+                t.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [p.grad.clone() for p in m.parameters()]
+        other.zero_grad()
+        other(x).backward(g)
+        assert all(torch.equal(a, p.grad) for a, p in zip(got, other.parameters())), seed
+    assert alive is not None
