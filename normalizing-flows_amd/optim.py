@@ -128,7 +128,8 @@ def muon_update(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=Tru
 
 class Muon(torch.optim.Optimizer):
     """muon_update over the parameters' gradients; state 'momentum_buffer' (float32).  Takes weight matrices only: give
-    biases and norm vectors to another optimizer."""
+    biases and norm vectors to another optimizer.  A step captured into a graph keeps the options that it was captured with, and
+    does not announce its writes: call nf.invalidate_weight_caches() after a replay before eager calls of the layers."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0., steps=5, eps=1e-7):
         _check_number('lr', lr, 0)
@@ -160,6 +161,9 @@ class Muon(torch.optim.Optimizer):
                     raise RuntimeError('Muon does not support sparse gradients')
                 state = self.state[p]
                 if 'momentum_buffer' not in state:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError('the first Muon step of a parameter makes its momentum buffer, which a captured step '
+                                           'would clear at every replay: take one step before capturing')
                     state['momentum_buffer'] = torch.zeros_like(p, memory_format=torch.contiguous_format)
                 by_device.setdefault(p.device, []).append((p, p.grad, state['momentum_buffer']))
             for entries in by_device.values():

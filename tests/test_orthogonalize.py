@@ -589,3 +589,35 @@ def test_forward_mode_is_refused():
             with pytest.raises(NotImplementedError, match='tangent'):
                 nf.muon_update(*args, lr=0.1)
     assert not p.any() and not m.any()
+
+
+@pytest.mark.gpu
+def test_captured_optimizer_step():
+    """The first step makes the momentum buffers: recorded into a graph they would be cleared at every replay, so that is refused.
+    Later steps replay with the same bits as eager ones, the momentum carried on."""
+    ps = [torch.nn.Parameter(gradients(s, 3, 0.1)) for s in ((70, 40), (20, 30))]
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    opt, eager = nf.Muon(ps, lr=0.1), nf.Muon(qs, lr=0.1)
+    for i, (p, q) in enumerate(zip(ps, qs)):
+        p.grad = gradients(p.shape, i)
+        q.grad = p.grad.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match='one step before'):
+            opt.step()
+        kept = ps[0].grad + 1
+    graph.replay()
+    assert torch.equal(kept, ps[0].grad + 1) and all(torch.equal(p, q) for p, q in zip(ps, qs))
+    opt.step()
+    eager.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for seed in range(4):
+        for i, (p, q) in enumerate(zip(ps, qs)):
+            p.grad.copy_(gradients(p.shape, 10 * seed + i))
+            q.grad.copy_(p.grad)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager.step()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs)), seed
