@@ -447,3 +447,62 @@ def test_capture_after_a_warm_up_whose_graph_lives(held):
         other(x).backward(g)
         assert all(torch.equal(a, p.grad) for a, p in zip(got, other.parameters())), seed
     assert alive is not None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kind', TYPES, ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize('rows,n', [(70001, 64), (33000, 200), (4500, 1031), (8500, 1100), (3001, 2048), (1100, 4500), (1100, 9000),
+                                    (1100, 16384), (600, 16385)])
+def test_more_rows_than_workgroups(rows, n, kind):
+    """Every kernel's loop over rows goes round more than once, the last time for a part of the workgroups or of their rows."""
+    x, w, b, g = (t.cuda() for t in data(rows, n, kind, seed=rows + n))
+    want = bounds(x, w, b, g, kind)
+    xd, wd, bd = x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+    out = nf.layer_norm(xd, wd, bd)
+    with torch.no_grad():
+        assert torch.equal(nf.layer_norm(xd, wd, bd), out)
+    got = (out, *torch.autograd.grad(out, (xd, wd, bd), g))
+    for name, v, (exact, tol) in zip(('y', 'grad_x', 'grad_w', 'grad_b'), got, want):
+        assert bool(((v.double() - exact).abs() <= tol).all()), name
+    again = torch.autograd.grad(nf.layer_norm(xd, wd, bd), (xd, wd, bd), g)
+    assert all(torch.equal(p, q) for p, q in zip(got[1:], again))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('mode', ['f32', 'f16x2'])
+@pytest.mark.parametrize('context', [None, 3])
+def test_residual_net_away_from_the_corners_of_relu(context, mode, monkeypatch):
+    """Values and every parameter's gradient of the conditioner against the same network in float64, on inputs drawn again until
+    no pre-activation lies within 1e-4 of 0, across which the fp32 run cannot move: both take the same branches.
+
+    Tolerance: ten products, norms and sums forwards and as many backwards, each of at most 64 + 22 roundings 2^-24 of a sum's
+    magnitudes, which exceed the largest value by at most ten."""
+    seen = []
+    relu = torch.Tensor.relu
+    monkeypatch.setattr(torch.Tensor, 'relu', lambda t: (seen.append(t.detach().abs().min().item()), relu(t))[1])
+    torch.manual_seed(4)
+    net = nf.ResidualNet(6, 10, 32, context_features=context, num_blocks=2, use_layer_norm=True).cuda()
+    with torch.no_grad():
+        for p in net.parameters():
+            p.add_(0.2 * torch.randn_like(p))
+    for _ in range(60):
+        x = torch.randn(64, 6)
+        c = None if context is None else torch.randn(64, context)
+        seen.clear()
+        want, p = _plain_net(net, x.double(), None if c is None else c.double())
+        assert len(seen) == 4
+        if min(seen) > 1e-4:
+            break
+    assert min(seen) > 1e-4
+    g = torch.randn(64, 10)
+    grads = torch.autograd.grad(want, list(p.values()), g.double())
+    nf.set_matmul_dtype(mode)
+    try:
+        out = net(x.cuda(), None if c is None else c.cuda())
+        got = torch.autograd.grad(out, list(net.parameters()), g.cuda())
+    finally:
+        nf.set_matmul_dtype('f32')
+    tol = 10 * 20 * (64 + 22) * U
+    assert ((out.detach().cpu().double() - want).abs().max() <= tol * want.abs().max()).item()
+    for name, a, b in zip(p, got, grads):
+        assert (a.cpu().double() - b).abs().max() <= tol * b.abs().max(), name

@@ -621,3 +621,28 @@ def test_captured_optimizer_step():
         torch.cuda.synchronize()
         eager.step()
         assert all(torch.equal(p, q) for p, q in zip(ps, qs)), seed
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kind', [torch.float32, torch.bfloat16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize('shape', [(3, 2100, 2500), (3, 2500, 2100), (4, 2050, 2050)], ids=str)
+def test_the_largest_tiles_at_their_ends(shape, kind):
+    """Batches that fill the device with tiles of 8 x 4 cells, which cross the matrix's end in both directions."""
+    g = gradients(shape, 4).to(kind)
+    out = nf.orthogonalize(g)
+    check(out, g, kind)
+    assert torch.equal(nf.orthogonalize(g), out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shape', [(2100, 2500), (2500, 2100), (2051, 2303), (2303, 2051)], ids=str)
+def test_muon_with_the_largest_tiles(shape):
+    """Parameters in rows of whole 16 bytes and not, as they are and transposed."""
+    check_muon([shape] * 4, 6, lr=0.02, weight_decay=0.1)
+
+
+@pytest.mark.gpu
+def test_largest_tiles_far_below_eps():
+    g = gradients((4, 2050, 2050), 4)
+    for ratio in (1e-3, 1e-12):
+        check(nf.orthogonalize(g, eps=norm(g).max().item() / ratio), g, torch.float32, eps=norm(g).max().item() / ratio)
