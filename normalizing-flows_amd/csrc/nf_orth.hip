@@ -41,8 +41,8 @@ constexpr int MAX_GROUPS = 8;            // shapes in one sequence of launches
 constexpr int MAX_MATRICES = 48;         // matrices with pointers of their own (kernel arguments) in one sequence
 constexpr int NORM_STRIDE = 256;         // doubles of a matrix in the workspace's first part: ...
 constexpr int NORM_BLOCKS = NORM_STRIDE - 1;             // ... partial sums of its norm, and X0's raise
-constexpr int NORM_THREADS = 512;        // of its workgroups (256: 4096 x 1024 372 us instead of 363; 1024: a Muon step of five
-                                         // 256-wide layers 232 instead of 222)
+constexpr int NORM_THREADS = 512;        // of its workgroups (4096 x 1024: 354 us, with 256 363; with 1024 level: 352 there, 20 of
+                                         // 512 x 512 332 instead of 329; three runs of each in turn on one device)
 constexpr int64_t SEQUENCE_BYTES = (int64_t)8 << 30;     // of X's and the slots' cells of one sequence of more than one matrix
 
 // matrices of one shape
@@ -1173,8 +1173,17 @@ constexpr int CUS = 256;
 
 // rows of cells of a workgroup in a launch of X's products
 int cut_mix(Plan& plan, int64_t& tiles) {
-    // 8 x 4 cells read each operand less often, where the k loop is long enough to carry their start and end
-    if ((tiles = count_tiles(plan, 8, 4, false)) >= 2 * CUS && plan.g[0].sm >= 64 && plan.groups == 1) return 8;
+    // 8 x 4 cells read each operand less often than 4 x 4: 4096 x 4096 4060 us instead of 4185, eight of 2048 x 2048 4000 and 4170,
+    // the Muon step of two 4096 x 4096 and two 4096 x 2048 9226 and 9640.  But k loops below 64 cells do not carry their start
+    // and end (256 of 256 x 512: 1125 us, with 4 x 4 1076; 64 of 512 x 512 level), and two of them fill a CU, so a round of 512
+    // that is nearly empty costs more than that of smaller ones: three of 2100 x 2500, 540 tiles, 2190 and 2010 us; 612 tiles
+    // 2435 and 2378, 640 level, 648 5345 and 5500.  Of a single round a quarter may be empty: 378 tiles 2565 and 2453, 390 2568
+    // and 2676.
+    int least = plan.g[0].sm;
+    for (int k = 1; k < plan.groups; ++k) least = plan.g[k].sm < least ? plan.g[k].sm : least;
+    tiles = count_tiles(plan, 8, 4, false);
+    const int64_t places = (tiles + 2 * CUS - 1) / (2 * CUS) * (2 * CUS);
+    if (least >= 64 && tiles * 8 >= places * (places > 2 * CUS ? 5 : 6)) return 8;
     // 4 x 4 cells against 2 x 2: k loops of up to 24 cells leave a large tile's start and end uncovered until several follow each
     // other on a CU (300 x 3000: eight 275 us with 2 x 2, 309 with 4 x 4; 32 of 380 x 4000 1576 and 1384); longer ones carry
     // them (1800 x 1800: 596 and 503 us)
