@@ -4,7 +4,8 @@
 //   backward  u = g w:  grad_x = r (u - mean u - xh mean(u xh)),  grad_w = sum_rows g xh,  grad_b = sum_rows g
 //
 // Bound: memory.  A row is read once into registers; mean and variance come from there in two sums (the second over
-// x - mu, so a large common offset costs no digits), all of it in fp32 whatever the element type.  The backward pass
+// x - mu, where a large common offset costs no more than mu's own rounding: every x - mu is shifted by up to 2^-24 |mu| and
+// the rounding of the row's sum), all of it in fp32 whatever the element type.  The backward pass
 // reads x and g once and writes grad_x; the row sums of grad_w / grad_b ride along in registers of a fixed grid of
 // workgroups, whose partial sums a second launch adds in a fixed order (no atomics: the same inputs give the same bits).
 //
@@ -329,7 +330,9 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* __restri
     }
 }
 
-// rows longer than 1024 threads keep: one workgroup a row, three passes over it (the later ones mostly from cache)
+// rows longer than 1024 threads keep: one workgroup a row, three passes over it (the later ones mostly from cache).  Measured:
+// 8192 x 20000 fp32 508 us (2.6 TB/s), with the backward pass 1279; 16384 x 20000 bf16 1331 us (1.0 TB/s) and 2798.  Bound by the
+// latency of each pass's loads, of which a thread has one on its way.
 template <typename T>
 __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(const T* __restrict__ x, int64_t xs,
                                                              const float* __restrict__ w, const float* __restrict__ b,

@@ -901,8 +901,8 @@ __device__ __forceinline__ void store_both(char* cell, char* transposed, const f
 
 // The m x m side of a block of steps in one launch, for sides up to 128: a workgroup of eight waves per matrix, the operands of
 // a product in two places of the LDS, every matrix's own values in fp32 registers (a wave has up to two cells i <= j of each).
-// S comes as raw accumulators; T of alpha I + T goes to slot 0, scaled for MixOp.  Nine products of 128 x 128 take 27 us, bound by
-// the LDS, against nine launches of 5 us and more.
+// S comes as raw accumulators; T of alpha I + T goes to slot 0, scaled for MixOp.  A block of two steps has five products of 128 x 128, of
+// three nine (27 us, against nine launches of 5 us and more): ten cells each on eight waves, so two waves have two of them while six wait.
 template <int SM>
 __global__ __launch_bounds__(512) void orth_chain_kernel(Plan plan, int block, int done, const double* __restrict__ norms,
                                                          const float* __restrict__ partial, char* __restrict__ ws) {
@@ -1245,8 +1245,9 @@ int cut_sym(Plan& plan, bool from_x, bool raw, int64_t& workgroups, int64_t& flo
 // largest singular values (their factor is near a^-j of it).  Frobenius errors measured against 64 bits, m >= 64, spectra
 // from flat to four decades: 1.3e-6 to 5.9e-6 step by step (fp32 products: 1.3e-6 to 5.1e-6), at most 1.2 times that with
 // two steps first, 2e-6 to 7.5e-6 with three and two.  So fp32 results and the Muon step (`exact`) get the first, 16-bit
-// results, whose own rounding is 2e-4 and more, the second.  Below m = 64 (few rounding errors to average) and where X is not
-// wide, step by step.
+// results, whose own rounding is 2e-4 and more, the second.  (The Muon step of five layers 784 -> 512 takes 1845 us; with three
+// and two 1332, with three and single ones 1587, which on a spectrum of one strong direction over noise is 2 to 4 times
+// further off than fp32 products.)  Below m = 64 (few rounding errors to average) and where X is not wide, step by step.
 int next_block(const Plan& plan, bool exact, int done, int steps) {
     double wide = 0, square = 0;
     for (int k = 0; k < plan.groups; ++k) {
